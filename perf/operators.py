@@ -164,7 +164,6 @@ def prepare(case, seed):
         qkv = torch.randn(t, (hq + 2 * hkv) * d, generator=gen, device="cuda").to(dtype)
         st["v"] = qkv[:, (hq + hkv) * d:].view(t, hkv, d)                                     # where the projection left it
         st["cu_seqlens"] = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device="cuda")
-        st["max_len"] = max(lens)
     return st
 
 
@@ -283,7 +282,7 @@ def run(st):
         if op == "attend":
             return quant_cache.kv4_attend(st["q"], st["pool"], st["req_to_token"], st["req_pool_indices"], st["seq_lens"],
                                           sm_scale=st["sm_scale"], rope_base=st["base"])
-        return prompt.prompt_attend(st["q"], st["k"], st["v"], st["cu_seqlens"], st["max_len"], sm_scale=st["sm_scale"])
+        return prompt.prompt_attend(st["q"], st["k"], st["v"], st["cu_seqlens"], sm_scale=st["sm_scale"])
     return {"norm": _plain_norm, "cache": _plain_cache, "attend": _plain_attend, "prompt": _plain_prompt}[op](st)
 
 
