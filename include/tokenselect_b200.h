@@ -334,6 +334,158 @@ typedef struct ts_attend_static_args {
 
 int ts_attend_rows_static(const ts_attend_static_args* args);
 
+/*
+ * A cache held in 4 bits.  A pool row keeps one token's K and V of every KV head; per KV head it is
+ *   K codes [head_dim/2] | V codes [head_dim/2] | K scales [head_dim/16] | V scales [head_dim/16]
+ * = 9*head_dim/8 bytes (144 at head_dim 128, against 512 in bf16).  Codes are 4-bit floats (E2M1: 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives), element 2i in the lower half of byte i; sixteen consecutive elements share one 8-bit
+ * scale (E4M3).  With the pool's scale g (k_scale or v_scale, a power of two, the same in every call on a pool):
+ *   scale = E4M3(min(max|x| / (6 g), 448)), code = E2M1(x / (g * scale)), value = code * scale * g
+ * both rounded to nearest, ties to the even code; the codes of a block whose scale rounds to 0 are 0.  A block with an
+ * infinity or a NaN reads back as NaN.  Every value is exact in bf16 and in fp32 (while g keeps it in their normal range),
+ * so a row read back and written again keeps its codes.  Keys are kept un-rotated, as in the bf16 pools.
+ *
+ * These calls take no handle and keep nothing between calls: any number of them may run at the same time, on any
+ * streams and in any captured graphs, as long as the caller orders writes and reads of the same rows.
+ * `device` is the ordinal that the pointers live on; it need not be the current one.  `status`, if not NULL, is a device
+ * int that the kernels set to the code of an error they find (it is never cleared here).
+ */
+typedef struct ts_quant_rows_args {
+    uint32_t struct_size;          /* sizeof(ts_quant_rows_args), checked */
+    int32_t device;
+    int32_t dtype;                 /* TS_DTYPE_* of k and v */
+    int32_t hkv;                   /* KV heads, 1 .. 1024 */
+    int32_t head_dim;              /* 64 or 128 */
+    int32_t count;                 /* rows; 0 does nothing */
+    void* k;                       /* row i, head h at k + i*k_stride + h*head_dim (elements); read by write, written by read */
+    void* v;
+    int64_t k_stride;              /* elements between rows, >= hkv*head_dim */
+    int64_t v_stride;
+    const int32_t* rows;           /* [count] pool rows */
+    void* pool;                    /* [pool_rows, hkv, 9*head_dim/8] bytes, start on a multiple of 16 */
+    int64_t pool_rows;
+    float k_scale, v_scale;        /* powers of two, 2^-32 .. 2^32 */
+    int32_t* status;
+    void* stream;                  /* cudaStream_t */
+} ts_quant_rows_args;
+
+/* Quantise `count` rows into the pool.  A row outside [0, pool_rows) is skipped and reported (TS_ERR_BAD_SLOT).  A pool row
+ * that is listed twice in one call is left with a mixture of the rows given for it. */
+int ts_quant_write(const ts_quant_rows_args* args);
+
+/* Read `count` rows back.  A row outside [0, pool_rows) gives zeros and is reported (TS_ERR_BAD_SLOT). */
+int ts_quant_read(const ts_quant_rows_args* args);
+
+/*
+ * Decode attention of a ragged batch over such a pool: request b attends to the rows
+ * req_to_token[req_pool_indices[b]][0 .. seq_lens[b]) -- all its tokens, or a list that a selection left; entry j sits at
+ * position j and is rotated there, the query at position seq_lens[b]-1 (as in ts_decode_layer's attention; angles are
+ * products of the whole position with a 64-bit frequency).  Query head h reads KV head h / (hq/hkv).
+ * A request of length 0 gets zeros.  A length below 0 or above max_ctx, or a request slot outside [0, max_reqs), gives zeros
+ * and is reported (TS_ERR_BAD_LENGTH); a row outside the pool counts as a row of zeros and is reported (TS_ERR_BAD_SLOT).
+ * In bf16 the rotated keys and queries and the softmax weights enter the products in fp16 (the queries scaled by a power of
+ * two into its range), all sums are fp32; in fp32 everything is fp32.
+ * `workspace` holds the partial results of one call (ts_quant_attend_workspace() bytes, any contents): calls that may run
+ * at the same time need one each.
+ */
+typedef struct ts_quant_attend_args {
+    uint32_t struct_size;          /* sizeof(ts_quant_attend_args), checked */
+    int32_t device;
+    int32_t dtype;                 /* TS_DTYPE_* of q and out */
+    int32_t batch;                 /* 0 .. 1024; 0 does nothing */
+    int32_t hq;                    /* query heads; hq / hkv <= 8 */
+    int32_t hkv;
+    int32_t head_dim;              /* 64 or 128 */
+    int32_t max_reqs;              /* rows of req_to_token */
+    const void* q;                 /* [batch, hq*head_dim], un-rotated; q and out on any element */
+    const void* pool;              /* [pool_rows, hkv, 9*head_dim/8] bytes, start on a multiple of 16 */
+    int64_t pool_rows;
+    const int32_t* req_to_token;   /* [max_reqs, stride] */
+    int64_t req_to_token_stride;   /* elements between rows */
+    int64_t max_ctx;               /* entries of a row that may be read */
+    const int32_t* req_pool_indices; /* [batch] */
+    const int32_t* seq_lens;       /* [batch] */
+    void* out;                     /* [batch, hq*head_dim] */
+    float sm_scale;                /* > 0 */
+    float logit_cap;               /* soft cap, used when > 0 */
+    double rope_base;
+    double rope_scale;
+    float k_scale, v_scale;        /* powers of two, 2^-32 .. 2^32 */
+    void* workspace;               /* start on a multiple of 16 */
+    size_t workspace_bytes;
+    int32_t* status;
+    void* stream;
+} ts_quant_attend_args;
+
+int ts_quant_attend_workspace(int32_t device, int32_t batch, int32_t hq, int32_t head_dim, size_t* bytes);
+int ts_quant_attend(const ts_quant_attend_args* args);
+
+/*
+ * RMS norm of every query and key head and the rotation of both, in one pass over them:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight        (no norm where the weight is NULL)
+ *   (y_i, y_{i+head_dim/2}) turned by position * rope_base^(-2i/head_dim) / rope_scale    (no rotation where positions is NULL)
+ * in fp32, rounded once.  k_plain, if not NULL, takes the normed keys before the rotation: what a cache of un-rotated keys
+ * keeps.  Outputs are contiguous [tokens, heads, head_dim]; an output may be the (contiguous) input of the same name.
+ */
+typedef struct ts_norm_rotate_args {
+    uint32_t struct_size;          /* sizeof(ts_norm_rotate_args), checked */
+    int32_t device;
+    int32_t dtype;                 /* TS_DTYPE_* of all tensors and weights */
+    int32_t tokens;                /* 0 does nothing */
+    int32_t hq, hkv;               /* 1 .. 1024 each */
+    int32_t head_dim;              /* 64 or 128 */
+    float eps;
+    const void* q;                 /* token t, head h at q + t*q_stride + h*head_dim (elements) */
+    const void* k;
+    int64_t q_stride;
+    int64_t k_stride;
+    const int32_t* positions;      /* [tokens] or NULL */
+    const void* q_weight;          /* [head_dim] or NULL */
+    const void* k_weight;          /* [head_dim] or NULL */
+    double rope_base;
+    double rope_scale;
+    void* q_out;
+    void* k_out;
+    void* k_plain;                 /* or NULL */
+    void* stream;
+} ts_norm_rotate_args;
+
+int ts_norm_rotate(const ts_norm_rotate_args* args);
+
+/*
+ * Causal attention of whole prompts: `batch` sequences packed one behind the other, sequence b being the tokens
+ * cu_seqlens[b] .. cu_seqlens[b+1]-1; token i attends to the tokens of its own sequence up to itself.  q and k come already
+ * rotated (ts_norm_rotate).  Query head h reads KV head h / (hq/hkv).  Lengths of zero and one are lengths like any other.
+ * cu_seqlens is read on the device; a bound outside [0, tokens] or below the one before it ends the sequence there and is
+ * reported (TS_ERR_BAD_LENGTH).  Rows of `out` that belong to no sequence (those behind the last one among them) are left as
+ * they were.  No value of one sequence reaches another, infinities and NaN included; inside
+ * a sequence they reach the tokens that attend to them.
+ * In bf16 the softmax weights enter the second product in bf16, all sums are fp32; in fp32 everything is fp32.
+ * bf16: q, k, v start on multiples of 16 bytes and their strides are multiples of 8 elements; out starts on a multiple of
+ * 16 bytes.  fp32: on multiples of 16 bytes, strides multiples of 4 elements.  (TS_ERR_INVALID_ARG otherwise.)
+ */
+typedef struct ts_prompt_args {
+    uint32_t struct_size;          /* sizeof(ts_prompt_args), checked */
+    int32_t device;
+    int32_t dtype;                 /* TS_DTYPE_* of q, k, v and out */
+    int32_t tokens;                /* rows of q, k, v and out; 0 does nothing */
+    int32_t batch;                 /* sequences, 0 .. 4096 */
+    int32_t hq, hkv;               /* hq a multiple of hkv */
+    int32_t head_dim;              /* 64 or 128 */
+    float sm_scale;                /* > 0 */
+    float logit_cap;               /* soft cap, used when > 0 */
+    const void* q;                 /* token t, head h at q + t*q_stride + h*head_dim (elements) */
+    const void* k;
+    const void* v;
+    int64_t q_stride, k_stride, v_stride;
+    const int32_t* cu_seqlens;     /* [batch+1] */
+    void* out;                     /* [tokens, hq, head_dim] */
+    int32_t* status;
+    void* stream;
+} ts_prompt_args;
+
+int ts_prompt_attend(const ts_prompt_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,7 +26,8 @@ EXPORTS = [
     "ts_destroy", "ts_reset_request", "ts_decode_layer", "ts_tp_prepare", "ts_tp_score_vote",
     "ts_tp_select_attend", "ts_get_counters", "ts_last_error", "ts_last_cuda_error", "ts_debug_read",
     "ts_launch_count", "ts_timing_begin", "ts_timing_end", "ts_attend_rows_static", "ts_tp_symmetric_bytes", "ts_tp_attach_peers",
-    "ts_extend_chunk",
+    "ts_extend_chunk", "ts_quant_write", "ts_quant_read", "ts_quant_attend_workspace", "ts_quant_attend", "ts_norm_rotate",
+    "ts_prompt_attend",
 ]
 
 
@@ -79,6 +80,49 @@ class TsAttendStaticArgs(C.Structure):
     ]
 
 
+class TsQuantRowsArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("hkv", C.c_int32),
+        ("head_dim", C.c_int32), ("count", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("rows", C.c_void_p), ("pool", C.c_void_p),
+        ("pool_rows", C.c_int64), ("k_scale", C.c_float), ("v_scale", C.c_float), ("status", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class TsQuantAttendArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("batch", C.c_int32),
+        ("hq", C.c_int32), ("hkv", C.c_int32), ("head_dim", C.c_int32), ("max_reqs", C.c_int32),
+        ("q", C.c_void_p), ("pool", C.c_void_p), ("pool_rows", C.c_int64), ("req_to_token", C.c_void_p),
+        ("req_to_token_stride", C.c_int64), ("max_ctx", C.c_int64), ("req_pool_indices", C.c_void_p),
+        ("seq_lens", C.c_void_p), ("out", C.c_void_p), ("sm_scale", C.c_float), ("logit_cap", C.c_float),
+        ("rope_base", C.c_double), ("rope_scale", C.c_double), ("k_scale", C.c_float), ("v_scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class TsNormRotateArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("tokens", C.c_int32),
+        ("hq", C.c_int32), ("hkv", C.c_int32), ("head_dim", C.c_int32), ("eps", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+        ("positions", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("rope_base", C.c_double),
+        ("rope_scale", C.c_double), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("k_plain", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class TsPromptArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("tokens", C.c_int32),
+        ("batch", C.c_int32), ("hq", C.c_int32), ("hkv", C.c_int32), ("head_dim", C.c_int32),
+        ("sm_scale", C.c_float), ("logit_cap", C.c_float), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("cu_seqlens", C.c_void_p),
+        ("out", C.c_void_p), ("status", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -116,6 +160,12 @@ def load() -> C.CDLL:
     lib.ts_tp_symmetric_bytes.argtypes = [C.POINTER(TsConfig), C.POINTER(C.c_size_t)]
     lib.ts_tp_attach_peers.argtypes = [H, C.POINTER(C.c_uint64), C.c_int32]
     lib.ts_extend_chunk.argtypes = [H, C.POINTER(TsExtendArgs)]
+    for name in ("ts_quant_write", "ts_quant_read"):
+        getattr(lib, name).argtypes = [C.POINTER(TsQuantRowsArgs)]
+    lib.ts_quant_attend_workspace.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]
+    lib.ts_quant_attend.argtypes = [C.POINTER(TsQuantAttendArgs)]
+    lib.ts_norm_rotate.argtypes = [C.POINTER(TsNormRotateArgs)]
+    lib.ts_prompt_attend.argtypes = [C.POINTER(TsPromptArgs)]
     if lib.ts_abi_version() != TS_ABI_VERSION:
         raise RuntimeError("libtokenselect_b200.so was built from a different header; rebuild it")
     _lib = lib

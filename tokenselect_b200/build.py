@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libtokenselect_b200.so")
 OBJ_DIR = os.path.join(HERE, "build")
-SOURCES = ["api.cu", "prep.cu", "fused.cu", "attend.cu", "attend_static.cu", "extend.cu"]
+SOURCES = ["api.cu", "prep.cu", "fused.cu", "attend.cu", "attend_static.cu", "extend.cu", "quant.cu", "quant_attend.cu", "norm_rotate.cu", "prompt.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xptxas", "-v",

@@ -1,0 +1,165 @@
+// ts_norm_rotate: RMS norm of every query and key head and the rotation of both in one pass.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w,   (y_i, y_{i+D/2}) -> (y_i cos - y_{i+D/2} sin, y_{i+D/2} cos + y_i sin)
+//
+// What bounds it: HBM (a row is read once, written once, a key row twice) and, for a few tokens, the launch.  Eight lanes
+// hold one (token, head) row: lane l the elements [P l, P l + P) of both halves (P = D/16), that is both members of its
+// rotation pairs, so the rotation exchanges nothing and the norm three shuffles.  Each thread evaluates the D/16 angles it
+// needs itself: an integer product each (rope.cuh), and in bf16 the fast sine and cosine, whose 2^-20 is far below the
+// output's 2^-9.  No table, no shared memory, no barrier: a block's rows are independent.
+#include "ptx.cuh"
+#include "rope.cuh"
+
+namespace ts {
+namespace {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormLanes = 8;                                  // lanes a row
+
+struct NormParams {
+    const void* q;
+    const void* k;
+    long long q_stride, k_stride;
+    const int* positions;
+    const void* q_weight;
+    const void* k_weight;
+    void* q_out;
+    void* k_out;
+    void* k_plain;
+    int hq, heads;                                             // heads = hq + hkv
+    long long rows;                                            // tokens * heads
+    float eps;
+    TurnFreqs freqs;
+};
+
+// P consecutive elements; WIDE: every row and every pointer is aligned to them.
+template <typename T, int P, bool WIDE>
+__device__ __forceinline__ void load_row(const T* src, float (&x)[P]) {
+    if constexpr (WIDE) {
+        constexpr int kBytes = P * (int)sizeof(T);
+        constexpr int kStep = kBytes < 16 ? kBytes : 16, kPer = kStep / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kBytes / kStep; ++i) {
+            alignas(16) T raw[kPer];
+            if constexpr (kStep == 16) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + i * kPer);
+            else *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src + i * kPer);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) x[i * kPer + e] = to_f32<T>(raw[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] = to_f32<T>(src[e]);
+    }
+}
+template <typename T, int P, bool WIDE>
+__device__ __forceinline__ void store_row(T* dst, const float (&x)[P]) {
+    if constexpr (WIDE) {
+        constexpr int kBytes = P * (int)sizeof(T);
+        constexpr int kStep = kBytes < 16 ? kBytes : 16, kPer = kStep / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kBytes / kStep; ++i) {
+            alignas(16) T raw[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) raw[e] = from_f32<T>(x[i * kPer + e]);
+            if constexpr (kStep == 16) *reinterpret_cast<uint4*>(dst + i * kPer) = *reinterpret_cast<const uint4*>(raw);
+            else *reinterpret_cast<uint2*>(dst + i * kPer) = *reinterpret_cast<const uint2*>(raw);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) dst[e] = from_f32<T>(x[e]);
+    }
+}
+
+template <typename T, int D, bool WIDE>
+__global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_constant__ NormParams p) {
+    constexpr int P = D / 2 / kNormLanes;
+    const int lane = threadIdx.x % kNormLanes;
+    const long long row = (long long)blockIdx.x * (kNormThreads / kNormLanes) + threadIdx.x / kNormLanes;
+    const bool mine = row < p.rows;                            // the others keep their warp's shuffles company
+    const long long t = mine ? row / p.heads : 0;
+    const int h = mine ? (int)(row - t * p.heads) : 0;
+    const bool is_q = h < p.hq;
+    const int hh = is_q ? h : h - p.hq;
+    const T* src = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_stride : reinterpret_cast<const T*>(p.k) + t * p.k_stride) +
+                   (long long)hh * D + P * lane;
+    const T* w = reinterpret_cast<const T*>(is_q ? p.q_weight : p.k_weight);
+    wait_for_predecessor();
+    float lo[P], hi[P];
+    load_row<T, P, WIDE>(src, lo);
+    load_row<T, P, WIDE>(src + D / 2, hi);
+    if (p.q_weight != nullptr || p.k_weight != nullptr) {      // uniform: whether any row of the launch is normed
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < P; ++e) sum += lo[e] * lo[e] + hi[e] * hi[e];
+#pragma unroll
+        for (int off = 1; off < kNormLanes; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (w != nullptr) {
+            const float r = rsqrtf(sum * (1.f / D) + p.eps);
+            float a[P], b[P];
+            load_row<T, P, WIDE>(w + P * lane, a);
+            load_row<T, P, WIDE>(w + D / 2 + P * lane, b);
+#pragma unroll
+            for (int e = 0; e < P; ++e) { lo[e] = lo[e] * r * a[e]; hi[e] = hi[e] * r * b[e]; }
+        }
+    }
+    if (!mine) return;
+    const long long at = (is_q ? t * p.hq + hh : t * (p.heads - p.hq) + hh) * D + P * lane;
+    if (!is_q && p.k_plain != nullptr) {
+        store_row<T, P, WIDE>(reinterpret_cast<T*>(p.k_plain) + at, lo);
+        store_row<T, P, WIDE>(reinterpret_cast<T*>(p.k_plain) + at + D / 2, hi);
+    }
+    if (p.positions != nullptr) {
+        const long long pos = p.positions[t];
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            const float2 cs = sizeof(T) == 2 ? cos_sin_fast(pos, p.freqs.f[P * lane + e]) : cos_sin(pos, p.freqs.f[P * lane + e]);
+            const float x = lo[e], y = hi[e];
+            lo[e] = x * cs.x - y * cs.y;
+            hi[e] = y * cs.x + x * cs.y;
+        }
+    }
+    T* out = reinterpret_cast<T*>(is_q ? p.q_out : p.k_out) + at;
+    store_row<T, P, WIDE>(out, lo);
+    store_row<T, P, WIDE>(out + D / 2, hi);
+}
+
+template <typename T, int D>
+cudaError_t launch_norm_rotate(const NormParams& p, cudaStream_t stream) {
+    constexpr int kAlign = (D / 16) * (int)sizeof(T) < 16 ? (D / 16) * (int)sizeof(T) : 16;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.q_weight) |
+                           reinterpret_cast<uintptr_t>(p.k_weight) | reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out) |
+                           reinterpret_cast<uintptr_t>(p.k_plain) | (uintptr_t)(p.q_stride * sizeof(T)) | (uintptr_t)(p.k_stride * sizeof(T));
+    const dim3 grid((unsigned)((p.rows * kNormLanes + kNormThreads - 1) / kNormThreads));
+    return bits % kAlign == 0 ? launch_chained(norm_rotate_kernel<T, D, true>, grid, dim3(kNormThreads), 0, stream, p)
+                              : launch_chained(norm_rotate_kernel<T, D, false>, grid, dim3(kNormThreads), 0, stream, p);
+}
+
+}  // namespace
+}  // namespace ts
+
+extern "C" int ts_norm_rotate(const ts_norm_rotate_args* a) {
+    using namespace ts;
+    if (!a || a->struct_size != sizeof(ts_norm_rotate_args)) return TS_ERR_INVALID_ARG;
+    if (a->dtype != TS_DTYPE_BF16 && a->dtype != TS_DTYPE_F32) return TS_ERR_UNSUPPORTED;
+    if (a->head_dim != 64 && a->head_dim != 128) return TS_ERR_UNSUPPORTED;
+    if (a->tokens < 0 || a->hq < 1 || a->hkv < 1 || a->hq > 1024 || a->hkv > 1024) return TS_ERR_INVALID_ARG;
+    if (a->q_stride < (int64_t)a->hq * a->head_dim || a->k_stride < (int64_t)a->hkv * a->head_dim) return TS_ERR_INVALID_ARG;
+    if (!(a->eps >= 0.f)) return TS_ERR_INVALID_ARG;
+    if (a->positions && (!(a->rope_base > 0.0) || !(a->rope_scale > 0.0))) return TS_ERR_INVALID_ARG;
+    if (a->tokens == 0) return TS_OK;
+    if (!a->q || !a->k || !a->q_out || !a->k_out) return TS_ERR_INVALID_ARG;
+    const DeviceScope scope(a->device);
+    if (!scope.ok) return TS_ERR_CUDA;
+    NormParams p;
+    p.q = a->q; p.k = a->k; p.q_stride = a->q_stride; p.k_stride = a->k_stride;
+    p.positions = a->positions; p.q_weight = a->q_weight; p.k_weight = a->k_weight;
+    p.q_out = a->q_out; p.k_out = a->k_out; p.k_plain = a->k_plain;
+    p.hq = a->hq; p.heads = a->hq + a->hkv; p.rows = (long long)a->tokens * p.heads; p.eps = a->eps;
+    if (p.rows > (1ll << 31) * (kNormThreads / kNormLanes) - kNormThreads) return TS_ERR_INVALID_ARG;      // blocks of one launch
+    if (a->positions) p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
+    cudaError_t e;
+    if (a->dtype == TS_DTYPE_BF16) e = a->head_dim == 128 ? launch_norm_rotate<__nv_bfloat16, 128>(p, s) : launch_norm_rotate<__nv_bfloat16, 64>(p, s);
+    else e = a->head_dim == 128 ? launch_norm_rotate<float, 128>(p, s) : launch_norm_rotate<float, 64>(p, s);
+    return e == cudaSuccess ? TS_OK : TS_ERR_CUDA;
+}

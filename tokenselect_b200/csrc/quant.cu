@@ -1,0 +1,181 @@
+// ts_quant_write, ts_quant_read: rows of a cache held in 4 bits, quantised as they are written and read back.
+//
+// Per block of sixteen elements x: scale = E4M3(min(max|x| / (6 g), 448)), code = E2M1(x / (g scale)), value = code scale g.
+//
+// What bounds both: HBM (a bf16 row of 2 KB at eight heads becomes 1152 bytes with its V), and for the rows of a decode
+// step the launch.  One thread takes one block: 32 bytes of bf16 or 64 of fp32 on one side, eight bytes of codes and one
+// scale on the other, so the maximum needs no exchange and neighbouring lanes touch neighbouring bytes on both sides.
+//
+// Rounding is decided exactly.  g is a power of two, so x / g is exact; max|x| / 6 is IEEE-divided, and a quotient that
+// lies beside a border of E4M3 does not round onto it (a border has five significant bits, so the dividend beside six times
+// it is at least two thirds of a unit of the quotient's last place away).  Borders of E2M1 times a scale have at most
+// seven significant bits: x either is on one, and then the quotient is exact, or at least 0.53 units of its last place off.
+#include "quant.cuh"
+#include "rope.cuh"
+
+namespace ts {
+namespace {
+
+constexpr int kRowsThreads = 256;
+
+struct QuantRowsParams {
+    void* k;
+    void* v;
+    long long k_stride, v_stride;
+    const int* rows;
+    unsigned char* pool;
+    long long pool_rows;
+    long long blocks;                                          // count * hkv * 2 * head_dim/16
+    int hkv;
+    float k_scale, v_scale;
+    int* status;
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_block(const T* src, float (&x)[kQuantBlock]) {
+    if constexpr (WIDE) {
+        constexpr int kPer = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kQuantBlock / kPer; ++i) {
+            alignas(16) T raw[kPer];
+            *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + i * kPer);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) x[i * kPer + e] = to_f32<T>(raw[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kQuantBlock; ++e) x[e] = to_f32<T>(src[e]);
+    }
+}
+
+// The block's codes in `w`; returns its scale.
+__device__ __forceinline__ uint32_t quantise_block(const float (&x)[kQuantBlock], float g, uint2& w) {
+    uint32_t top = 0;                                          // largest magnitude; as bits, so that NaN counts as the largest
+#pragma unroll
+    for (int e = 0; e < kQuantBlock; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    w = make_uint2(0u, 0u);
+    if (top >= 0x7f800000u) return 0x7fu;                      // an infinity or a NaN: the scale is NaN
+    const float inv_g = 1.f / g;
+    const uint32_t scale = f32_to_e4m3(fminf(__fdiv_rn(__uint_as_float(top) * inv_g, 6.f), 448.f));
+    if (scale == 0) return 0;
+    const float s = e4m3_to_f32(scale);
+    float y[2][8];
+#pragma unroll
+    for (int e = 0; e < kQuantBlock; ++e) y[e >> 3][e & 7] = __fdiv_rn(x[e] * inv_g, s);
+    w = make_uint2(f32x8_to_e2m1(y[0]), f32x8_to_e2m1(y[1]));
+    return scale;
+}
+
+struct BlockPlace { int i, head, part; bool is_v; };           // row of the call, head, block of the head
+template <int D>
+__device__ __forceinline__ BlockPlace block_place(long long b, int hkv) {
+    constexpr int kParts = D / kQuantBlock;
+    BlockPlace r;
+    r.part = (int)(b % kParts);
+    const long long u = b / kParts;                            // (row, K or V, head)
+    r.head = (int)(u % hkv);
+    const long long w = u / hkv;
+    r.is_v = (w & 1) != 0;
+    r.i = (int)(w >> 1);
+    return r;
+}
+
+template <typename T, int D, bool WIDE>
+__global__ void __launch_bounds__(kRowsThreads) quant_write_kernel(const QuantRowsParams p) {
+    using Row = QuantRow<D>;
+    const long long b = (long long)blockIdx.x * kRowsThreads + threadIdx.x;
+    wait_for_predecessor();
+    if (b >= p.blocks) return;
+    const BlockPlace at = block_place<D>(b, p.hkv);
+    const int row = p.rows[at.i];
+    if (row < 0 || row >= p.pool_rows) { report(p.status, TS_ERR_BAD_SLOT); return; }
+    const T* src = at.is_v ? reinterpret_cast<const T*>(p.v) + at.i * p.v_stride : reinterpret_cast<const T*>(p.k) + at.i * p.k_stride;
+    float x[kQuantBlock];
+    load_block<T, WIDE>(src + at.head * D + at.part * kQuantBlock, x);
+    uint2 w;
+    const uint32_t scale = quantise_block(x, at.is_v ? p.v_scale : p.k_scale, w);
+    unsigned char* dst = p.pool + ((long long)row * p.hkv + at.head) * Row::kBytes;
+    *reinterpret_cast<uint2*>(dst + (at.is_v ? Row::kV : 0) + at.part * 8) = w;
+    dst[(at.is_v ? Row::kVScales : Row::kKScales) + at.part] = (unsigned char)scale;
+}
+
+template <typename T, int D, bool WIDE>
+__global__ void __launch_bounds__(kRowsThreads) quant_read_kernel(const QuantRowsParams p) {
+    using Row = QuantRow<D>;
+    const long long b = (long long)blockIdx.x * kRowsThreads + threadIdx.x;
+    wait_for_predecessor();
+    if (b >= p.blocks) return;
+    const BlockPlace at = block_place<D>(b, p.hkv);
+    const int row = p.rows[at.i];
+    uint2 w = make_uint2(0u, 0u);
+    uint32_t scale = 0;
+    if (row >= 0 && row < p.pool_rows) {
+        const unsigned char* src = p.pool + ((long long)row * p.hkv + at.head) * Row::kBytes;
+        w = *reinterpret_cast<const uint2*>(src + (at.is_v ? Row::kV : 0) + at.part * 8);
+        scale = src[(at.is_v ? Row::kVScales : Row::kKScales) + at.part];
+    } else {
+        report(p.status, TS_ERR_BAD_SLOT);
+    }
+    const float s = e4m3_to_f32(scale) * (at.is_v ? p.v_scale : p.k_scale);
+    T* dst = (at.is_v ? reinterpret_cast<T*>(p.v) + at.i * p.v_stride : reinterpret_cast<T*>(p.k) + at.i * p.k_stride) +
+             at.head * D + at.part * kQuantBlock;
+    uint32_t h[2][4];
+    e2m1x8_to_f16(w.x, h[0]);
+    e2m1x8_to_f16(w.y, h[1]);
+    alignas(16) T out[kQuantBlock];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float2 f = half2_to_float2(h[e >> 2][e & 3]);
+        out[2 * e] = from_f32<T>(f.x * s);
+        out[2 * e + 1] = from_f32<T>(f.y * s);
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(out) / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(out)[i];
+    } else {
+#pragma unroll
+        for (int e = 0; e < kQuantBlock; ++e) dst[e] = out[e];
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch_rows_t(const QuantRowsParams& p, bool write, cudaStream_t stream) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | (uintptr_t)(p.k_stride * sizeof(T)) |
+                           (uintptr_t)(p.v_stride * sizeof(T));
+    const bool wide = bits % 16 == 0;
+    const dim3 grid((unsigned)((p.blocks + kRowsThreads - 1) / kRowsThreads)), block(kRowsThreads);
+    if (write) return wide ? launch_chained(quant_write_kernel<T, D, true>, grid, block, 0, stream, p)
+                           : launch_chained(quant_write_kernel<T, D, false>, grid, block, 0, stream, p);
+    return wide ? launch_chained(quant_read_kernel<T, D, true>, grid, block, 0, stream, p)
+                : launch_chained(quant_read_kernel<T, D, false>, grid, block, 0, stream, p);
+}
+
+int quant_rows(const ts_quant_rows_args* a, bool write) {
+    if (!a || a->struct_size != sizeof(ts_quant_rows_args)) return TS_ERR_INVALID_ARG;
+    if (a->dtype != TS_DTYPE_BF16 && a->dtype != TS_DTYPE_F32) return TS_ERR_UNSUPPORTED;
+    if (a->head_dim != 64 && a->head_dim != 128) return TS_ERR_UNSUPPORTED;
+    if (a->hkv < 1 || a->hkv > 1024 || a->count < 0 || a->pool_rows < 1) return TS_ERR_INVALID_ARG;
+    if (a->k_stride < (int64_t)a->hkv * a->head_dim || a->v_stride < (int64_t)a->hkv * a->head_dim) return TS_ERR_INVALID_ARG;
+    if (!power_of_two(a->k_scale) || !power_of_two(a->v_scale)) return TS_ERR_INVALID_ARG;
+    if (a->count == 0) return TS_OK;
+    if (!a->k || !a->v || !a->rows || !a->pool || reinterpret_cast<uintptr_t>(a->pool) % 16 != 0) return TS_ERR_INVALID_ARG;
+    const DeviceScope scope(a->device);
+    if (!scope.ok) return TS_ERR_CUDA;
+    QuantRowsParams p;
+    p.k = a->k; p.v = a->v; p.k_stride = a->k_stride; p.v_stride = a->v_stride; p.rows = a->rows;
+    p.pool = static_cast<unsigned char*>(a->pool); p.pool_rows = a->pool_rows; p.hkv = a->hkv;
+    p.blocks = (long long)a->count * a->hkv * 2 * (a->head_dim / kQuantBlock);
+    if (p.blocks > ((1ll << 31) - 1) * kRowsThreads) return TS_ERR_INVALID_ARG;
+    p.k_scale = a->k_scale; p.v_scale = a->v_scale; p.status = a->status;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
+    cudaError_t e;
+    if (a->dtype == TS_DTYPE_BF16) e = a->head_dim == 128 ? launch_rows_t<__nv_bfloat16, 128>(p, write, s) : launch_rows_t<__nv_bfloat16, 64>(p, write, s);
+    else e = a->head_dim == 128 ? launch_rows_t<float, 128>(p, write, s) : launch_rows_t<float, 64>(p, write, s);
+    return e == cudaSuccess ? TS_OK : TS_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace ts
+
+extern "C" int ts_quant_write(const ts_quant_rows_args* a) { return ts::quant_rows(a, true); }
+extern "C" int ts_quant_read(const ts_quant_rows_args* a) { return ts::quant_rows(a, false); }
