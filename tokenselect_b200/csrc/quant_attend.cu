@@ -6,6 +6,8 @@
 // units [U c / G, U (c+1) / G), whatever the lengths; it keeps a running maximum and sum per head and leaves one partial
 // result per request it meets, in slot c + request (unique, because both grow along the sequence).  A second kernel joins
 // them.  Every kernel derives the pieces from the lengths alone: nothing is planned on the host, which does not know them.
+#include <limits.h>
+
 #include "quant.cuh"
 #include "rope.cuh"
 
@@ -226,6 +228,393 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 }
 
 // ------------------------------------------------------------------------------------------------
+// Tensor cores: bf16
+// ------------------------------------------------------------------------------------------------
+// What bounds it: HBM in the long run (144 bytes a row and head for 512 a group-of-four bf16 flops), and close behind it the
+// instructions that turn 4-bit codes into operands; so the layout spares those.
+//
+// A warp takes one KV head; its up to eight query heads are the N of m16n8k16 products in fp16.  S^T = K Q^T has sixteen
+// keys as M: a key row's codes, read eight bytes at a time, ARE the A fragments of a thread once converted, because a
+// product over d does not mind in which order it meets the d's -- thread t of a quad simply owns elements [16 t, 16 t + 16) of
+// both halves of the head (both members of its rotation pairs, and two scales in all).  O^T = V^T P^T has sixteen d as M:
+// thread g owns the d of one scale block, and two keys' codes are interleaved as 4-bit fields (four instructions for sixteen
+// elements) so that one conversion gives the pair (key, key + 1) that a fragment register holds.  S^T becomes the B
+// fragment of the second product with one movmatrix per eight keys.
+//
+// Rotation.  R(n-1) q . R(j0 + i) k = (R(n-1-j0) q) . (R(i) k): per macro tile of 128 keys the query is turned in fp32 by its
+// exact distance to the tile's first key, and a key only by its place i in the tile, from a table of 128 rows of cosines and
+// sines in fp16 that stays in shared memory.  No table grows with the context, and the far angles stay exact.
+//
+// Rows arrive through a ring of five stages of sixteen rows per warp (cp.async, 16 bytes a piece: 144 pieces a stage), so
+// a warp waits for nobody else until its piece is done.  Shared memory holds rows without padding: the order in which the
+// sixteen keys are given to the sixteen M rows makes every read of eight-byte fragments free of bank conflicts.
+constexpr int kQtWarps = 16, kQtThreads = 32 * kQtWarps;
+constexpr int kQtStages = 5;
+constexpr int kQtMacro = 8;                                    // units of a macro tile
+
+template <int D>
+struct QuantTcSmem {
+    unsigned char ring[kQtWarps][kQtStages][kUnit * QuantRow<D>::kBytes];
+    uint4 turn[kQtMacro * kUnit][D / 8];                       // per key of a macro tile: cosines, sines of the pairs, fp16
+    float2 base[kQtWarps][D / 2];                              // per warp: (cos, sin) of the query's distance to the tile
+    float2 ml[kQtWarps][8];
+    int start[kQaMaxBatch + 1];
+};
+
+// Key of a stage that M row m of a fragment stands for: rows 0..7 the even keys, 8..15 the odd ones, in an order in which
+// the four rows of a half-warp's read lie 32 bytes apart modulo 128, for K (rows g) and for V (rows 2t and 2t + 1) alike.
+__device__ __forceinline__ int key_of(int m) { return ((m & 4) ? 8 + (((m & 3) * 2) ^ 2) : (m & 3) * 2) + (m >> 3); }
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t neg2(uint32_t a) { return a ^ 0x80008000u; }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_piece(uint32_t dst, const unsigned char* src, int bytes) {      // zeros behind `bytes`
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A thread's eight (D = 64: four) bytes of a row's codes.
+template <int D>
+__device__ __forceinline__ void load_words(const unsigned char* src, uint32_t (&w)[D / 64]) {
+    if constexpr (D == 128) { const uint2 x = *reinterpret_cast<const uint2*>(src); w[0] = x.x; w[1] = x.y; }
+    else w[0] = *reinterpret_cast<const uint32_t*>(src);
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __grid_constant__ QuantAttendParams p) {
+    using Row = QuantRow<D>;
+    constexpr int HALF = D / 2, NW = D / 64, MT = D / 16, PIECE = D / 8;      // words a half, M tiles of O, bytes of a copy
+    constexpr int kPieces = kUnit * 9, kRounds = (kPieces + 31) / 32;
+    extern __shared__ __align__(16) unsigned char dyn[];
+    QuantTcSmem<D>& sm = *reinterpret_cast<QuantTcSmem<D>*>(dyn);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+    // The turns of a macro tile's keys.  16-byte unit 4 c + t (c: cosines' then sines' words) holds what thread t reads; the units
+    // of odd keys are exchanged by fours so that a read of two keys by eight lanes meets eight different bank groups.
+    {
+        const int pair = threadIdx.x % HALF, owner = pair / (D / 8), r = pair % (D / 8);
+        const unsigned long long f = p.freqs.f[pair];
+        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit; i += kQtThreads / HALF) {
+            const float2 cs = cos_sin_fast(i, f);
+            __half* row = reinterpret_cast<__half*>(sm.turn[i]);
+            const int swap = (i & 1) * (D == 128 ? 4 : 2);
+            // D = 128: a thread's 16 pairs are two units of cosines and two of sines; D = 64: its 8 pairs one of each
+            const int uc = ((r >> 3) * 4 + owner) ^ swap, us = ((NW + (r >> 3)) * 4 + owner) ^ swap;
+            row[uc * 8 + (r & 7)] = __float2half_rn(cs.x);
+            row[us * 8 + (r & 7)] = __float2half_rn(cs.y);
+        }
+    }
+    wait_for_predecessor();
+    count_units(p, sm.start);                                  // ends with a barrier: the table is complete too
+    const int units = sm.start[p.batch], pieces = used_pieces(units, p.pieces);
+    if ((int)blockIdx.x >= pieces) return;
+    const int u_end = piece_start(units, blockIdx.x + 1, pieces);
+    const int hpc = (p.hkv + gridDim.y - 1) / gridDim.y, share = kQtWarps / hpc;      // KV heads of a CTA, warps of a head
+    const int my_head = warp % hpc, kv = blockIdx.y * hpc + my_head, my_share = warp / hpc;
+    const bool busy = my_share < share && kv < p.hkv;
+    const unsigned char* head_pool = p.pool + (long long)kv * Row::kBytes;
+    const long long row_bytes = (long long)p.hkv * Row::kBytes;
+    unsigned char* ring = sm.ring[warp][0];
+    const uint32_t ring_at = smem_u32(ring);
+    const unsigned long long f0 = p.freqs.f[lane], f1 = D == 128 ? p.freqs.f[(lane + 32) % HALF] : 0ull;
+
+    int u0 = piece_start(units, blockIdx.x, pieces);
+    while (u0 < u_end) {
+        const int b = request_of(sm.start, p.batch, u0);
+        const int n = p.seq_lens[b], first = sm.start[b], u1 = min(u_end, sm.start[b + 1]);
+        const int* table = p.rtt + (long long)p.req_pool_indices[b] * p.rtt_stride;
+        // macro tiles of `per` units go round the warps of a head
+        const int per = min(kQtMacro, (u1 - u0 + share - 1) / share);
+        int steps = 0;                                         // units of this warp
+        if (busy) {
+            const int round = share * per, full = (u1 - u0) / round, rest = u1 - u0 - full * round;
+            steps = full * per + min(per, max(0, rest - my_share * per));
+        }
+        float o[MT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+
+        if (steps > 0) {
+            // the query of head g, a quad's thread holding its pairs; scaled by a power of two to below 2
+            uint32_t q_lo[4 * NW], q_hi[4 * NW];
+            float unit_scale;
+            {
+                const bool real = g < p.group;
+                const __nv_bfloat16* qh = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((long long)b * p.hq + kv * p.group + (real ? g : 0)) * D + t * (D / 8);
+                const bool aligned = (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 4 * NW; ++i) {
+                    q_lo[i] = real ? load_bf16_pair(qh + 2 * i, aligned) : 0u;
+                    q_hi[i] = real ? load_bf16_pair(qh + HALF + 2 * i, aligned) : 0u;
+                    top = max(top, max(max(q_lo[i] & 0x7fffu, (q_lo[i] >> 16) & 0x7fffu), max(q_hi[i] & 0x7fffu, (q_hi[i] >> 16) & 0x7fffu)));
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const uint32_t ex = min(max(top >> 7, 1u), 253u);             // biased exponent of the largest element
+                const float down = __uint_as_float((254u - ex) << 23);
+                unit_scale = __uint_as_float(ex << 23) * p.sm_scale;
+#pragma unroll
+                for (int i = 0; i < 4 * NW; ++i) {
+                    q_lo[i] = pack_bf16x2(__uint_as_float(q_lo[i] << 16) * down, __uint_as_float(q_lo[i] & 0xffff0000u) * down);
+                    q_hi[i] = pack_bf16x2(__uint_as_float(q_hi[i] << 16) * down, __uint_as_float(q_hi[i] & 0xffff0000u) * down);
+                }
+            }
+            // a column of S^T is a query head: this thread's columns are heads 2t and 2t + 1
+            const float per_log = CAP ? 1.f : kLog2e;
+            const float mul0 = __shfl_sync(0xffffffffu, unit_scale, 8 * t) * per_log, mul1 = __shfl_sync(0xffffffffu, unit_scale, 8 * t + 4) * per_log;
+
+            auto unit_at = [&](int s) { const int mt = s / per; return u0 + (mt * share + my_share) * per + (s - mt * per); };
+            auto row_ids = [&](int s) {                        // lane l and l + 16: row l of the unit, or none
+                if (s >= steps) return INT_MIN;
+                const int r = (unit_at(s) - first) * kUnit + (lane & 15);
+                return r < n ? __ldg(table + r) : INT_MIN;
+            };
+            auto request = [&](int stage, int ids) {
+                const bool bad = ids != INT_MIN && (ids < 0 || ids >= p.pool_rows);
+                if (bad) report(p.status, TS_ERR_BAD_SLOT);
+                const int row = bad || ids == INT_MIN ? -1 : ids;
+#pragma unroll
+                for (int k = 0; k < kRounds; ++k) {
+                    const int piece = lane + 32 * k, r = piece / 9, c = piece - 9 * r;
+                    const int id = __shfl_sync(0xffffffffu, row, r & 15);
+                    if (32 * k + 32 <= kPieces || piece < kPieces)
+                        copy_piece<PIECE>(ring_at + stage * (kUnit * Row::kBytes) + piece * PIECE, head_pool + max(id, 0) * row_bytes + c * PIECE, id < 0 ? 0 : PIECE);
+                }
+                copies_commit();
+            };
+            {
+                int ids[kQtStages];
+#pragma unroll
+                for (int s = 0; s < kQtStages; ++s) ids[s] = row_ids(s);
+#pragma unroll
+                for (int s = 0; s < kQtStages; ++s) request(s, ids[s]);
+            }
+            int next_a = row_ids(kQtStages), next_b = row_ids(kQtStages + 1);
+            uint32_t qa[4 * NW], qb[4 * NW];
+            int stage = 0, in_macro = 0;                       // units of the macro tile done
+
+            for (int s = 0; s < steps;) {
+                const int cnt = min(min(2, per - in_macro), steps - s);
+                const int row0 = (unit_at(s) - first) * kUnit;  // first key of this step
+                if (in_macro == 0) {
+                    // the query, turned by its distance to the tile's first key
+                    __syncwarp();
+                    const int slot = lane / (D / 8) * (D / 8) + (((lane % (D / 8)) / 2 ^ ((lane / (D / 8)) * 2)) % (D / 16)) * 2 + (lane & 1);
+                    sm.base[warp][slot] = cos_sin_fast(n - 1 - row0, f0);
+                    if (D == 128) {
+                        const int l2 = lane + 32, slot2 = l2 / 16 * 16 + (((l2 % 16) / 2 ^ ((l2 / 16) * 2)) % 8) * 2 + (l2 & 1);
+                        sm.base[warp][slot2] = cos_sin_fast(n - 1 - row0, f1);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4 * NW; ++i) {
+                        const float4 cs = *reinterpret_cast<const float4*>(&sm.base[warp][t * (D / 8) + ((i ^ (t * 2)) % (D / 16)) * 2]);
+                        const float x0 = __uint_as_float(q_lo[i] << 16), x1 = __uint_as_float(q_lo[i] & 0xffff0000u);
+                        const float y0 = __uint_as_float(q_hi[i] << 16), y1 = __uint_as_float(q_hi[i] & 0xffff0000u);
+                        qa[i] = pack2(x0 * cs.x - y0 * cs.y, x1 * cs.z - y1 * cs.w);
+                        qb[i] = pack2(y0 * cs.x + x0 * cs.y, y1 * cs.z + x1 * cs.w);
+                    }
+                }
+                if (cnt == 2) copies_wait<kQtStages - 2>(); else copies_wait<kQtStages - 1>();
+                __syncwarp();
+
+                float sc[2][4];
+                const int stage1 = stage + 1 == kQtStages ? 0 : stage + 1;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
+                    if (j < cnt) {
+                        const unsigned char* st = ring + (j == 0 ? stage : stage1) * (kUnit * Row::kBytes);
+                        uint32_t a_lo[2][4 * NW], a_hi[2][4 * NW];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const int key = key_of(g + 8 * r);
+                            const unsigned char* row = st + key * Row::kBytes;
+                            uint32_t lo[NW], hi[NW];
+                            load_words<D>(row + t * 4 * NW, lo);
+                            load_words<D>(row + D / 4 + t * 4 * NW, hi);
+                            const int blk = t * (D / 8) / kQuantBlock;
+                            const uint32_t two = e4m3x2_to_f16(row[Row::kKScales + blk] | (uint32_t)row[Row::kKScales + D / 32 + blk] << 8);
+                            const uint32_t sl = __byte_perm(two, two, 0x1010), sh = __byte_perm(two, two, 0x3232);
+                            const int i = (in_macro + j) * kUnit + key, swap = (i & 1) * (D == 128 ? 4 : 2);
+#pragma unroll
+                            for (int w = 0; w < NW; ++w) {
+                                uint32_t x[4], y[4];
+                                e2m1x8_to_f16(lo[w], x);
+                                e2m1x8_to_f16(hi[w], y);
+                                const uint4 c4 = sm.turn[i][(4 * w + t) ^ swap], s4 = sm.turn[i][(4 * (NW + w) + t) ^ swap];
+                                const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t xs = mul2(x[e], sl), ys = mul2(y[e], sh);
+                                    a_lo[r][4 * w + e] = fma2(neg2(ys), sn[e], mul2(xs, c[e]));
+                                    a_hi[r][4 * w + e] = fma2(xs, sn[e], mul2(ys, c[e]));
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int ks = 0; ks < 4 * NW; ++ks) {
+                            const uint32_t a[4] = {a_lo[0][ks], a_lo[1][ks], a_hi[0][ks], a_hi[1][ks]};
+                            mma_f16_16816(sc[j], a, qa[ks], qb[ks]);
+                        }
+                        const int left = n - (row0 + j * kUnit);
+                        if (left < kUnit) {                    // the request's last unit
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                if (key_of(g + 8 * r) >= left) { sc[j][2 * r] = -INFINITY; sc[j][2 * r + 1] = -INFINITY; }
+                        }
+                        if (CAP) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = sc[j][e] * ((e & 1) ? mul1 : mul0);
+                                sc[j][e] = x == -INFINITY ? x : p.logit_cap * tanhf(x / p.logit_cap) * kLog2e;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[j][e] = -INFINITY;
+                    }
+                }
+                const float k0 = CAP ? 1.f : mul0, k1 = CAP ? 1.f : mul1;
+                float x0 = fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2])) * k0;
+                float x1 = fmaxf(fmaxf(sc[0][1], sc[0][3]), fmaxf(sc[1][1], sc[1][3])) * k1;
+#pragma unroll
+                for (int off = 4; off <= 16; off <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
+                }
+                // the reference maximum moves only when a row grew by more than 2^8: weights stay below 256
+                if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f)) {
+                    const float n0 = fmaxf(fmaxf(m0, x0), -1e30f), n1 = fmaxf(fmaxf(m1, x1), -1e30f);
+                    const float c0 = exp2_fast(m0 - n0), c1 = exp2_fast(m1 - n1);
+                    m0 = n0, m1 = n1;
+                    l0 *= c0, l1 *= c1;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) { o[i][0] *= c0; o[i][1] *= c1; o[i][2] *= c0; o[i][3] *= c1; }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (j >= cnt) break;
+                    float pe[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pe[e] = exp2_fast(fmaf(sc[j][e], (e & 1) ? k1 : k0, (e & 1) ? -m1 : -m0));
+                    l0 += pe[0] + pe[2];
+                    l1 += pe[1] + pe[3];
+                    const uint32_t b0 = transpose8(pack2(pe[0], pe[1])), b1 = transpose8(pack2(pe[2], pe[3]));
+                    const unsigned char* st = ring + (j == 0 ? stage : stage1) * (kUnit * Row::kBytes);
+                    const unsigned char* ra = st + key_of(2 * t) * Row::kBytes;           // keys of the fragment's columns 2t, 2t+1,
+                    const unsigned char* rb = st + key_of(2 * t + 1) * Row::kBytes;       // and one row further on 2t+8, 2t+9
+                    const int blk = g * (D / 8) / kQuantBlock;
+                    uint32_t a[2][MT], h[2][MT];               // even and odd d of the thread's block; keys (2t, 2t+1), (2t+8, 2t+9)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        uint32_t wa[NW], wb[NW];
+                        load_words<D>(ra + r * Row::kBytes + Row::kV + g * 4 * NW, wa);
+                        load_words<D>(rb + r * Row::kBytes + Row::kV + g * 4 * NW, wb);
+                        const uint32_t s2 = e4m3x2_to_f16(ra[r * Row::kBytes + Row::kVScales + blk] | (uint32_t)rb[r * Row::kBytes + Row::kVScales + blk] << 8);
+#pragma unroll
+                        for (int w = 0; w < NW; ++w) {
+                            uint32_t x[4], y[4];
+                            e2m1x8_to_f16((wa[w] & 0x0f0f0f0fu) | ((wb[w] << 4) & 0xf0f0f0f0u), x);
+                            e2m1x8_to_f16(((wa[w] >> 4) & 0x0f0f0f0fu) | (wb[w] & 0xf0f0f0f0u), y);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { a[r][4 * w + e] = mul2(x[e], s2); h[r][4 * w + e] = mul2(y[e], s2); }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const uint32_t f[4] = {a[0][i], h[0][i], a[1][i], h[1][i]};
+                        mma_f16_16816(o[i], f, b0, b1);
+                    }
+                }
+                __syncwarp();                                  // every lane has read the stages that are requested into next
+                request(stage, next_a);
+                if (cnt == 2) {
+                    request(stage1, next_b);
+                    next_a = row_ids(s + kQtStages + 2);
+                    next_b = row_ids(s + kQtStages + 3);
+                    stage = stage1 + 1 == kQtStages ? 0 : stage1 + 1;
+                } else {
+                    next_a = next_b;
+                    next_b = row_ids(s + kQtStages + 2);
+                    stage = stage1;
+                }
+                s += cnt;
+                in_macro += cnt;
+                if (in_macro == per) in_macro = 0;
+            }
+            copies_wait<0>();
+#pragma unroll
+            for (int off = 4; off <= 16; off <<= 1) {
+                l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+                l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+            }
+        }
+        // join the warps of a head; the ring is free
+        __syncwarp();
+        float* mine = reinterpret_cast<float*>(ring);          // [8][D]
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            *reinterpret_cast<float2*>(mine + (2 * t) * D + g * (D / 8) + 2 * i) = make_float2(o[i][0], o[i][2]);
+            *reinterpret_cast<float2*>(mine + (2 * t + 1) * D + g * (D / 8) + 2 * i) = make_float2(o[i][1], o[i][3]);
+        }
+        if (g == 0) { sm.ml[warp][2 * t] = make_float2(m0, l0); sm.ml[warp][2 * t + 1] = make_float2(m1, l1); }
+        __syncthreads();
+        if (busy) {
+            const long long slot = blockIdx.x + b;
+            for (int i = my_share * 32 + lane; i < p.group * D; i += share * 32) {
+                const int h = i / D, d = i - h * D;
+                float mm = -1e30f;
+                for (int w = 0; w < share; ++w) mm = fmaxf(mm, sm.ml[w * hpc + my_head][h].x);
+                float sum = 0.f, l = 0.f;
+                for (int w = 0; w < share; ++w) {
+                    const float2 ml = sm.ml[w * hpc + my_head][h];
+                    const float weight = exp2_fast(ml.x - mm);
+                    sum += reinterpret_cast<const float*>(sm.ring[w * hpc + my_head][0])[h * D + d] * weight;
+                    l += ml.y * weight;
+                }
+                const long long at = slot * p.hq + kv * p.group + h;
+                p.part_o[at * D + d] = sum;
+                if (d == 0) p.part_ml[at] = make_float2(mm, l);
+            }
+        }
+        __syncthreads();
+        u0 = u1;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
 // Join the partial results: grid (hq, batch), one warp per partial in flight
 // ------------------------------------------------------------------------------------------------
 constexpr int kQmThreads = 256;
@@ -304,17 +693,30 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
     }
 }
 
-// Pieces the sequence of units is cut into.
-int plain_pieces(int sms) { return 4 * sms; }
+// Pieces the sequence of units is cut into: for the tensor cores one CTA per SM, sixteen warps over at most sixteen KV heads
+// each; for the CUDA cores what fits an SM.
+int tc_head_blocks(int hkv) { return (hkv + kQtWarps - 1) / kQtWarps; }
+int attend_pieces(int dtype, int hkv, int sms) {
+    return dtype == TS_DTYPE_BF16 ? (sms + tc_head_blocks(hkv) - 1) / tc_head_blocks(hkv) : 4 * sms;
+}
 
 size_t partial_bytes(int pieces, int batch, int hq, int d) { return (size_t)(pieces + batch) * hq * (d + 2) * sizeof(float); }
 
-template <typename T, int D>
+template <int D>
 cudaError_t launch_attend_plain(const QuantAttendParams& p, cudaStream_t stream) {
     const int nsub = (p.group + kQpHeads - 1) / kQpHeads, per_cta = kQpThreads / 32;
-    cudaError_t e = launch_chained(quant_attend_plain_kernel<T, D>, dim3(p.pieces, (p.hkv * nsub + per_cta - 1) / per_cta), dim3(kQpThreads), 0, stream, p);
+    const cudaError_t e = launch_chained(quant_attend_plain_kernel<float, D>, dim3(p.pieces, (p.hkv * nsub + per_cta - 1) / per_cta), dim3(kQpThreads), 0, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_chained(quant_merge_kernel<T, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+    return launch_chained(quant_merge_kernel<float, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+}
+template <int D, bool CAP>
+cudaError_t launch_attend_tc(const QuantAttendParams& p, cudaStream_t stream) {
+    static SmemConfig configured = {};
+    cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP>, sizeof(QuantTcSmem<D>), configured);
+    if (e != cudaSuccess) return e;
+    e = launch_chained(quant_attend_tc_kernel<D, CAP>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), sizeof(QuantTcSmem<D>), stream, p);
+    if (e != cudaSuccess) return e;
+    return launch_chained(quant_merge_kernel<__nv_bfloat16, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
 }
 
 }  // namespace
@@ -326,7 +728,7 @@ extern "C" int ts_quant_attend_workspace(int32_t device, int32_t batch, int32_t 
     if (head_dim != 64 && head_dim != 128) return TS_ERR_UNSUPPORTED;
     const int sms = sms_of(device);
     if (sms <= 0) return TS_ERR_CUDA;
-    *bytes = partial_bytes(plain_pieces(sms), batch, hq, head_dim);
+    *bytes = partial_bytes(4 * sms, batch, hq, head_dim);      // the most that any type and head count takes
     return TS_OK;
 }
 
@@ -346,7 +748,7 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     if (reinterpret_cast<uintptr_t>(a->pool) % 16 != 0 || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return TS_ERR_INVALID_ARG;
     const int sms = sms_of(a->device);
     if (sms <= 0) return TS_ERR_CUDA;
-    const int pieces = plain_pieces(sms);
+    const int pieces = attend_pieces(a->dtype, a->hkv, sms);
     if (a->workspace_bytes < partial_bytes(pieces, a->batch, a->hq, a->head_dim)) return TS_ERR_CAPACITY;
     const DeviceScope scope(a->device);
     if (!scope.ok) return TS_ERR_CUDA;
@@ -362,7 +764,9 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;
-    if (a->dtype == TS_DTYPE_BF16) e = a->head_dim == 128 ? launch_attend_plain<__nv_bfloat16, 128>(p, s) : launch_attend_plain<__nv_bfloat16, 64>(p, s);
-    else e = a->head_dim == 128 ? launch_attend_plain<float, 128>(p, s) : launch_attend_plain<float, 64>(p, s);
+    const bool cap = a->logit_cap > 0.f;
+    if (a->dtype == TS_DTYPE_F32) e = a->head_dim == 128 ? launch_attend_plain<128>(p, s) : launch_attend_plain<64>(p, s);
+    else if (a->head_dim == 128) e = cap ? launch_attend_tc<128, true>(p, s) : launch_attend_tc<128, false>(p, s);
+    else e = cap ? launch_attend_tc<64, true>(p, s) : launch_attend_tc<64, false>(p, s);
     return e == cudaSuccess ? TS_OK : TS_ERR_CUDA;
 }
