@@ -245,37 +245,69 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 // exact distance to the tile's first key, and a key only by its place i in the tile, from a table of 128 rows of cosines and
 // sines in fp16 that stays in shared memory.  No table grows with the context, and the far angles stay exact.
 //
-// Rows arrive through a ring of five stages of sixteen rows per warp (cp.async, 16 bytes a piece: 144 pieces a stage), so
-// a warp waits for nobody else until its piece is done.  Shared memory holds rows without padding: the order in which the
-// sixteen keys are given to the sixteen M rows makes every read of eight-byte fragments free of bank conflicts.
-constexpr int kQtWarps = 16, kQtThreads = 32 * kQtWarps;
-constexpr int kQtStages = 5;
+// Rows arrive through rings in shared memory: the warps that take the same units (one per KV head) share one.  Four warps of
+// their own request the units in turn, all heads of the CTA at once.  With three heads or more that is one bulk copy a row,
+// sixteen by one instruction, which holds its warp for a microsecond whatever their number and size (measured, random rows, four
+// warps: 6.4 TB/s in rows of 1152 bytes, 4.2 in rows of 576, but 1.1 in rows of 144).  Narrower rows, and rows of D = 64 that lie off the
+// copies' 16-byte grid, come in cp.async pieces.  A row takes 16 bytes modulo 128 in shared memory, and the order in which
+// the sixteen keys are given to the sixteen M rows then makes every read of eight-byte fragments free of bank conflicts.
+// Eight computing warps with their operands in registers do as well as sixteen with some of them spilled.
+constexpr int kQtWarps = 8, kQtLoaders = 4, kQtThreads = 32 * (kQtWarps + kQtLoaders);
+constexpr int kQtBulkBytes = 400;                              // bulk copies for rows of at least this many
 constexpr int kQtMacro = 8;                                    // units of a macro tile
+// Stages of a ring: a step holds two while the two behind it arrive, so fewer than four would wait for themselves.
+constexpr int kQtMinStages = 4, kQtMaxStages = 8, kQtBytes = 232448;          // (dynamic shared memory)
 
 template <int D>
-struct QuantTcSmem {
-    unsigned char ring[kQtWarps][kQtStages][kUnit * QuantRow<D>::kBytes];
+struct QuantTcSmem {                                           // behind it: the heads' queries, then the rings
     uint4 turn[kQtMacro * kUnit][D / 8];                       // per key of a macro tile: cosines, sines of the pairs, fp16
     float2 base[kQtWarps][D / 2];                              // per warp: (cos, sin) of the query's distance to the tile
     float2 ml[kQtWarps][8];
+    uint64_t full[kQtWarps][kQtMaxStages], empty[kQtWarps][kQtMaxStages];
     int start[kQaMaxBatch + 1];
+    int pad[3];
 };
+// Bytes between the rows of `heads` heads in shared memory: 16 modulo 128.
+template <int D>
+__host__ __device__ __forceinline__ int row_pitch(int heads) {
+    const int bytes = heads * QuantRow<D>::kBytes;
+    return bytes + ((16 - bytes) & 127);
+}
+
+template <int D>
+constexpr bool rings_fit() {
+    for (int heads = 1; heads <= kQtWarps; ++heads) {
+        const int bytes = heads * QuantRow<D>::kBytes, pitch = bytes + ((16 - bytes) & 127);
+        if (kQtBytes - (int)sizeof(QuantTcSmem<D>) - heads * D * 16 < kQtMinStages * kUnit * pitch) return false;
+        if (kQtBytes - (int)sizeof(QuantTcSmem<D>) - heads * D * 16 < kQtWarps * 8 * D * 4) return false;       // the warps' results at the end
+    }
+    return true;
+}
+static_assert(rings_fit<128>() && rings_fit<64>(), "four stages for one warp of every head count");
+
+// Whether a phase is complete, without waiting for it (try_wait may suspend the warp for a while).
+__device__ __forceinline__ bool test_phase(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A wait of at most about a second; then the call's status says so, and the waits that follow give up at once.
+__device__ __forceinline__ void wait_phase(uint32_t bar, uint32_t parity, int* status, bool& dead) {
+    if (mbar_try_wait(bar, parity) || dead) return;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - t0 > kWaitCycles) { report(status, TS_ERR_DEVICE_TIMEOUT); dead = true; return; }
+}
 
 // Key of a stage that M row m of a fragment stands for: rows 0..7 the even keys, 8..15 the odd ones, in an order in which
 // the four rows of a half-warp's read lie 32 bytes apart modulo 128, for K (rows g) and for V (rows 2t and 2t + 1) alike.
 __device__ __forceinline__ int key_of(int m) { return ((m & 4) ? 8 + (((m & 3) * 2) ^ 2) : (m & 3) * 2) + (m >> 3); }
 
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t neg2(uint32_t a) { return a ^ 0x80008000u; }
+__device__ __forceinline__ __half2 as_half2(uint32_t a) { return *reinterpret_cast<const __half2*>(&a); }
+__device__ __forceinline__ uint32_t as_bits(__half2 a) { return *reinterpret_cast<const uint32_t*>(&a); }
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) { return as_bits(__hmul2(as_half2(a), as_half2(b))); }
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) { return as_bits(__hfma2(as_half2(a), as_half2(b), as_half2(c))); }
+__device__ __forceinline__ uint32_t fnma2(uint32_t a, uint32_t b, uint32_t c) { return as_bits(__hfma2(__hneg2(as_half2(a)), as_half2(b), as_half2(c))); }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -296,9 +328,6 @@ __device__ __forceinline__ void copy_piece(uint32_t dst, const unsigned char* sr
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // A thread's eight (D = 64: four) bytes of a row's codes.
 template <int D>
@@ -307,21 +336,21 @@ __device__ __forceinline__ void load_words(const unsigned char* src, uint32_t (&
     else w[0] = *reinterpret_cast<const uint32_t*>(src);
 }
 
-template <int D, bool CAP>
+// PIECE: 0, rows by bulk copies; 16 or 8, by pieces of that many bytes.
+template <int D, bool CAP, int PIECE>
 __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __grid_constant__ QuantAttendParams p) {
     using Row = QuantRow<D>;
-    constexpr int HALF = D / 2, NW = D / 64, MT = D / 16, PIECE = D / 8;      // words a half, M tiles of O, bytes of a copy
-    constexpr int kPieces = kUnit * 9, kRounds = (kPieces + 31) / 32;
+    constexpr int HALF = D / 2, NW = D / 64, MT = D / 16;      // words a half, M tiles of O
     extern __shared__ __align__(16) unsigned char dyn[];
     QuantTcSmem<D>& sm = *reinterpret_cast<QuantTcSmem<D>*>(dyn);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
     // The turns of a macro tile's keys.  16-byte unit 4 c + t (c: cosines' then sines' words) holds what thread t reads; the units
-    // of odd keys are exchanged by fours so that a read of two keys by eight lanes meets eight different bank groups.
+    // of odd keys are exchanged by halves so that a read of two keys by eight lanes meets eight different bank groups.
     {
         const int pair = threadIdx.x % HALF, owner = pair / (D / 8), r = pair % (D / 8);
         const unsigned long long f = p.freqs.f[pair];
-        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit; i += kQtThreads / HALF) {
+        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit && warp < kQtWarps; i += 32 * kQtWarps / HALF) {
             const float2 cs = cos_sin_fast(i, f);
             __half* row = reinterpret_cast<__half*>(sm.turn[i]);
             const int swap = (i & 1) * (D == 128 ? 4 : 2);
@@ -331,18 +360,37 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
             row[us * 8 + (r & 7)] = __float2half_rn(cs.y);
         }
     }
+    const int hpc = (p.hkv + gridDim.y - 1) / gridDim.y;       // KV heads of a CTA
+    const int head0 = blockIdx.y * hpc, heads = min(hpc, p.hkv - head0);
+    const int pitch = row_pitch<D>(hpc), stage_bytes = kUnit * pitch;
+    const int ring_space = kQtBytes - (int)sizeof(QuantTcSmem<D>) - hpc * D * 16;
+    const int share = min(kQtWarps / hpc, ring_space / (kQtMinStages * stage_bytes));           // warps of a head
+    uint4* queries = reinterpret_cast<uint4*>(dyn + sizeof(QuantTcSmem<D>));                   // [hpc][D/32][32]: pairs of a lane, bf16
+    unsigned char* rings = reinterpret_cast<unsigned char*>(queries + hpc * D);
+    const int stages = min(kQtMaxStages, ring_space / (share * stage_bytes));
+    const bool requests = warp >= kQtWarps;
+    const int my_head = warp % hpc, kv = head0 + my_head, my_share = warp / hpc;
+    const bool busy = !requests && my_share < share && my_head < heads;
+    if (threadIdx.x < share * stages) {
+        const int r = threadIdx.x / stages, i = threadIdx.x % stages;
+        mbar_init(smem_u32(&sm.full[r][i]), PIECE == 0 ? 1 : 32);
+        mbar_init(smem_u32(&sm.empty[r][i]), heads);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     wait_for_predecessor();
-    count_units(p, sm.start);                                  // ends with a barrier: the table is complete too
+    count_units(p, sm.start);                                  // ends with a barrier: the table and the barriers are complete too
     const int units = sm.start[p.batch], pieces = used_pieces(units, p.pieces);
     if ((int)blockIdx.x >= pieces) return;
     const int u_end = piece_start(units, blockIdx.x + 1, pieces);
-    const int hpc = (p.hkv + gridDim.y - 1) / gridDim.y, share = kQtWarps / hpc;      // KV heads of a CTA, warps of a head
-    const int my_head = warp % hpc, kv = blockIdx.y * hpc + my_head, my_share = warp / hpc;
-    const bool busy = my_share < share && kv < p.hkv;
-    const unsigned char* head_pool = p.pool + (long long)kv * Row::kBytes;
+    const unsigned char* head_pool = p.pool + (long long)head0 * Row::kBytes;
     const long long row_bytes = (long long)p.hkv * Row::kBytes;
-    unsigned char* ring = sm.ring[warp][0];
-    const uint32_t ring_at = smem_u32(ring);
+    const int width = heads * Row::kBytes;                     // bytes of a row that this CTA takes
+    unsigned char* ring = rings + min(my_share, share - 1) * stages * stage_bytes;
+    const uint32_t full = smem_u32(sm.full[min(my_share, share - 1)]), empty = smem_u32(sm.empty[min(my_share, share - 1)]);
+    int stage = 0;                                             // next stage to read
+    uint32_t phase = 0;                                        // parity of its barrier
+    int before = 0;                                            // a requesting warp's lane w: units of share w in the requests so far
+    bool dead = false;
     const unsigned long long f0 = p.freqs.f[lane], f1 = D == 128 ? p.freqs.f[(lane + 32) % HALF] : 0ull;
 
     int u0 = piece_start(units, blockIdx.x, pieces);
@@ -351,32 +399,98 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
         const int n = p.seq_lens[b], first = sm.start[b], u1 = min(u_end, sm.start[b + 1]);
         const int* table = p.rtt + (long long)p.req_pool_indices[b] * p.rtt_stride;
         // macro tiles of `per` units go round the warps of a head
-        const int per = min(kQtMacro, (u1 - u0 + share - 1) / share);
-        int steps = 0;                                         // units of this warp
-        if (busy) {
-            const int round = share * per, full = (u1 - u0) / round, rest = u1 - u0 - full * round;
-            steps = full * per + min(per, max(0, rest - my_share * per));
-        }
+        const int rounds = (u1 - u0 + share * kQtMacro - 1) / (share * kQtMacro), per = (u1 - u0 + share * rounds - 1) / (share * rounds);
+        auto units_of = [&](int w) {                           // of share w
+            const int round = share * per, whole = (u1 - u0) / round, rest = u1 - u0 - whole * round;
+            return whole * per + min(per, max(0, rest - w * per));
+        };
+        const int steps = busy ? units_of(my_share) : 0, skip = (share - 1) * per;
         float o[MT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
+        if (requests) {
+            // Lane w keeps the place of share w: unit `at` of its units, counted over all requests, goes into stage at % stages and is
+            // requested by warp at % 4 of these.  Lanes 16 (w & 1) + r of ahead[w / 2] hold the number of row r of this warp's next
+            // unit (or none), read when the one before was requested.
+            const int end = before + (lane < share ? units_of(lane) : 0);
+            int at = before + ((warp - kQtWarps - before) & (kQtLoaders - 1)), ahead[kQtWarps / 2];
+            auto unit_of = [&]() { const int k = at - before, m = k / per; return u0 + (m * share + lane) * per + k - m * per; };
+            auto read_ahead = [&](int w, int unit) {
+                const int r = (unit - first) * kUnit + (lane & 15);
+                const bool mine = lane >> 4 == (w & 1), some = unit < u1 && r < n;
+#pragma unroll
+                for (int i = 0; i < kQtWarps / 2; ++i)
+                    if (mine && w >> 1 == i) {
+                        if (some) ahead[i] = __ldg(table + r); else ahead[i] = INT_MIN;
+                    }
+            };
+            {
+                const int unit = unit_of();
+                for (int w = 0; w < share; ++w) read_ahead(w, __shfl_sync(0xffffffffu, unit, w));
+            }
+            long long idle_since = clock64();
+            while (__any_sync(0xffffffffu, at < end)) {
+                const int stage_in = at % stages;
+                const bool ready = at < end && (dead || test_phase(smem_u32(&sm.empty[lane % kQtWarps][stage_in]), (at / stages & 1) ^ 1));
+                unsigned todo = __ballot_sync(0xffffffffu, ready);
+                if (todo == 0) {
+                    if (clock64() - idle_since > kWaitCycles) { report(p.status, TS_ERR_DEVICE_TIMEOUT); dead = true; }
+                    dead = __any_sync(0xffffffffu, dead);
+                    continue;
+                }
+                for (; todo != 0; todo &= todo - 1) {
+                    const int w = __ffs(todo) - 1, to = __shfl_sync(0xffffffffu, stage_in, w);
+                    int pair = ahead[0];
+#pragma unroll
+                    for (int i = 1; i < kQtWarps / 2; ++i) pair = w >> 1 == i ? ahead[i] : pair;
+                    const int r = lane & 15, id = __shfl_sync(0xffffffffu, pair, (w & 1) * 16 + r);
+                    unsigned char* dst = rings + (w * stages + to) * stage_bytes;
+                    const uint32_t bar = smem_u32(&sm.full[w][to]);
+                    const bool bad = id != INT_MIN && (id < 0 || id >= p.pool_rows);
+                    if (bad) report(p.status, TS_ERR_BAD_SLOT);
+                    const bool some = !bad && id != INT_MIN;
+                    const unsigned char* src = head_pool + (some ? id * row_bytes : 0);
+                    if constexpr (PIECE == 0) {
+                        const unsigned rows = __ballot_sync(0xffffffffu, some) & 0xffffu;
+                        if (rows != 0xffffu) {                 // zeros where no row comes
+                            for (int i = 0; i < kUnit; ++i)
+                                if (!(rows >> i & 1))
+                                    for (int j = lane; j < width / 8; j += 32) reinterpret_cast<uint2*>(dst + i * pitch)[j] = make_uint2(0u, 0u);
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // a later copy into the stage comes behind them
+                            __syncwarp();
+                        }
+                        if (lane == 0) mbar_expect_tx(bar, __popc(rows) * width);
+                        __syncwarp();
+                        if (lane < 16 && some) bulk_g2s(smem_u32(dst + r * pitch), src, width, bar);
+                    } else {
+                        // two lanes a row, two neighbouring pieces at a time
+                        for (int j = (lane >> 4) * PIECE; j < width; j += 2 * PIECE) copy_piece<PIECE>(smem_u32(dst + r * pitch + j), src + (some ? j : 0), some ? PIECE : 0);
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                    }
+                    if (lane == w) at += kQtLoaders;
+                    const int unit = unit_of();
+                    read_ahead(w, __shfl_sync(0xffffffffu, unit, w));
+                }
+                idle_since = clock64();
+            }
+            before = end;
+        }
         if (steps > 0) {
-            // the query of head g, a quad's thread holding its pairs; scaled by a power of two to below 2
-            uint32_t q_lo[4 * NW], q_hi[4 * NW];
+            // the query of head g, of which a quad's thread turns its own pairs; scaled by a power of two to below 2
+            const bool real = g < p.group;
+            const __nv_bfloat16* qh = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((long long)b * p.hq + kv * p.group + (real ? g : 0)) * D + t * (D / 8);
+            const bool aligned = (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;
             float unit_scale;
             {
-                const bool real = g < p.group;
-                const __nv_bfloat16* qh = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((long long)b * p.hq + kv * p.group + (real ? g : 0)) * D + t * (D / 8);
-                const bool aligned = (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;
-                uint32_t top = 0;
+                uint32_t x[4 * NW], y[4 * NW], top = 0;
 #pragma unroll
                 for (int i = 0; i < 4 * NW; ++i) {
-                    q_lo[i] = real ? load_bf16_pair(qh + 2 * i, aligned) : 0u;
-                    q_hi[i] = real ? load_bf16_pair(qh + HALF + 2 * i, aligned) : 0u;
-                    top = max(top, max(max(q_lo[i] & 0x7fffu, (q_lo[i] >> 16) & 0x7fffu), max(q_hi[i] & 0x7fffu, (q_hi[i] >> 16) & 0x7fffu)));
+                    x[i] = real ? load_bf16_pair(qh + 2 * i, aligned) : 0u;           // heads beyond the group: zeros
+                    y[i] = real ? load_bf16_pair(qh + HALF + 2 * i, aligned) : 0u;
+                    top = max(top, max(max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu), max(y[i] & 0x7fffu, (y[i] >> 16) & 0x7fffu)));
                 }
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -385,47 +499,26 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 unit_scale = __uint_as_float(ex << 23) * p.sm_scale;
 #pragma unroll
                 for (int i = 0; i < 4 * NW; ++i) {
-                    q_lo[i] = pack_bf16x2(__uint_as_float(q_lo[i] << 16) * down, __uint_as_float(q_lo[i] & 0xffff0000u) * down);
-                    q_hi[i] = pack_bf16x2(__uint_as_float(q_hi[i] << 16) * down, __uint_as_float(q_hi[i] & 0xffff0000u) * down);
+                    x[i] = pack_bf16x2(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down);
+                    y[i] = pack_bf16x2(__uint_as_float(y[i] << 16) * down, __uint_as_float(y[i] & 0xffff0000u) * down);
+                }
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    // (the warps of a head write the same values to the same place)
+                    queries[(my_head * 2 * NW + w) * 32 + lane] = make_uint4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]);
+                    queries[(my_head * 2 * NW + NW + w) * 32 + lane] = make_uint4(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3]);
                 }
             }
             // a column of S^T is a query head: this thread's columns are heads 2t and 2t + 1
             const float per_log = CAP ? 1.f : kLog2e;
             const float mul0 = __shfl_sync(0xffffffffu, unit_scale, 8 * t) * per_log, mul1 = __shfl_sync(0xffffffffu, unit_scale, 8 * t + 4) * per_log;
 
-            auto unit_at = [&](int s) { const int mt = s / per; return u0 + (mt * share + my_share) * per + (s - mt * per); };
-            auto row_ids = [&](int s) {                        // lane l and l + 16: row l of the unit, or none
-                if (s >= steps) return INT_MIN;
-                const int r = (unit_at(s) - first) * kUnit + (lane & 15);
-                return r < n ? __ldg(table + r) : INT_MIN;
-            };
-            auto request = [&](int stage, int ids) {
-                const bool bad = ids != INT_MIN && (ids < 0 || ids >= p.pool_rows);
-                if (bad) report(p.status, TS_ERR_BAD_SLOT);
-                const int row = bad || ids == INT_MIN ? -1 : ids;
-#pragma unroll
-                for (int k = 0; k < kRounds; ++k) {
-                    const int piece = lane + 32 * k, r = piece / 9, c = piece - 9 * r;
-                    const int id = __shfl_sync(0xffffffffu, row, r & 15);
-                    if (32 * k + 32 <= kPieces || piece < kPieces)
-                        copy_piece<PIECE>(ring_at + stage * (kUnit * Row::kBytes) + piece * PIECE, head_pool + max(id, 0) * row_bytes + c * PIECE, id < 0 ? 0 : PIECE);
-                }
-                copies_commit();
-            };
-            {
-                int ids[kQtStages];
-#pragma unroll
-                for (int s = 0; s < kQtStages; ++s) ids[s] = row_ids(s);
-#pragma unroll
-                for (int s = 0; s < kQtStages; ++s) request(s, ids[s]);
-            }
-            int next_a = row_ids(kQtStages), next_b = row_ids(kQtStages + 1);
             uint32_t qa[4 * NW], qb[4 * NW];
-            int stage = 0, in_macro = 0;                       // units of the macro tile done
+            int in_macro = 0, unit = u0 + my_share * per;      // units of the macro tile done; the next one
 
             for (int s = 0; s < steps;) {
                 const int cnt = min(min(2, per - in_macro), steps - s);
-                const int row0 = (unit_at(s) - first) * kUnit;  // first key of this step
+                const int row0 = (unit - first) * kUnit;       // first key of this step
                 if (in_macro == 0) {
                     // the query, turned by its distance to the tile's first key
                     __syncwarp();
@@ -437,73 +530,83 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                     }
                     __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 4 * NW; ++i) {
-                        const float4 cs = *reinterpret_cast<const float4*>(&sm.base[warp][t * (D / 8) + ((i ^ (t * 2)) % (D / 16)) * 2]);
-                        const float x0 = __uint_as_float(q_lo[i] << 16), x1 = __uint_as_float(q_lo[i] & 0xffff0000u);
-                        const float y0 = __uint_as_float(q_hi[i] << 16), y1 = __uint_as_float(q_hi[i] & 0xffff0000u);
-                        qa[i] = pack2(x0 * cs.x - y0 * cs.y, x1 * cs.z - y1 * cs.w);
-                        qb[i] = pack2(y0 * cs.x + x0 * cs.y, y1 * cs.z + x1 * cs.w);
+                    for (int w = 0; w < NW; ++w) {
+                        const uint4 x4 = queries[(my_head * 2 * NW + w) * 32 + lane], y4 = queries[(my_head * 2 * NW + NW + w) * 32 + lane];
+                        const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 4 * w + e;
+                            const float4 cs = *reinterpret_cast<const float4*>(&sm.base[warp][t * (D / 8) + ((i ^ (t * 2)) % (D / 16)) * 2]);
+                            const float x0 = __uint_as_float(x[e] << 16), x1 = __uint_as_float(x[e] & 0xffff0000u);
+                            const float y0 = __uint_as_float(y[e] << 16), y1 = __uint_as_float(y[e] & 0xffff0000u);
+                            qa[i] = pack2(x0 * cs.x - y0 * cs.y, x1 * cs.z - y1 * cs.w);
+                            qb[i] = pack2(y0 * cs.x + x0 * cs.y, y1 * cs.z + x1 * cs.w);
+                        }
                     }
                 }
-                if (cnt == 2) copies_wait<kQtStages - 2>(); else copies_wait<kQtStages - 1>();
-                __syncwarp();
+                const int stage1 = stage + 1 == stages ? 0 : stage + 1;
+                wait_phase(full + 8 * stage, phase, p.status, dead);
+                if (cnt == 2) wait_phase(full + 8 * stage1, phase ^ (stage1 == 0), p.status, dead);
 
+                // S^T of the step's two units side by side (of a step with one unit, the second is whatever its stage holds, masked
+                // below): the products of one run while the other's operands are made
                 float sc[2][4];
-                const int stage1 = stage + 1 == kQtStages ? 0 : stage + 1;
+                const unsigned char* st[2] = {ring + stage * stage_bytes + my_head * Row::kBytes, ring + stage1 * stage_bytes + my_head * Row::kBytes};
+                uint32_t s_lo[2][2], s_hi[2][2];               // scales of the thread's two blocks, [unit][parity of the key]
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
-                    if (j < cnt) {
-                        const unsigned char* st = ring + (j == 0 ? stage : stage1) * (kUnit * Row::kBytes);
-                        uint32_t a_lo[2][4 * NW], a_hi[2][4 * NW];
+                    for (int r = 0; r < 2; ++r) {
+                        const unsigned char* row = st[j] + key_of(g + 8 * r) * pitch + Row::kKScales + t * (D / 8) / kQuantBlock;
+                        const uint32_t two = e4m3x2_to_f16(row[0] | (uint32_t)row[D / 32] << 8);
+                        s_lo[j][r] = __byte_perm(two, two, 0x1010);
+                        s_hi[j][r] = __byte_perm(two, two, 0x3232);
+                        sc[j][2 * r] = 0.f;
+                        sc[j][2 * r + 1] = 0.f;
+                    }
+                const int in_second = min(in_macro + 1, kQtMacro - 1);
+#pragma unroll
+                for (int w = 0; w < NW; ++w)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t a_lo[2][4], a_hi[2][4];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const int key = key_of(g + 8 * r);
-                            const unsigned char* row = st + key * Row::kBytes;
-                            uint32_t lo[NW], hi[NW];
-                            load_words<D>(row + t * 4 * NW, lo);
-                            load_words<D>(row + D / 4 + t * 4 * NW, hi);
-                            const int blk = t * (D / 8) / kQuantBlock;
-                            const uint32_t two = e4m3x2_to_f16(row[Row::kKScales + blk] | (uint32_t)row[Row::kKScales + D / 32 + blk] << 8);
-                            const uint32_t sl = __byte_perm(two, two, 0x1010), sh = __byte_perm(two, two, 0x3232);
-                            const int i = (in_macro + j) * kUnit + key, swap = (i & 1) * (D == 128 ? 4 : 2);
-#pragma unroll
-                            for (int w = 0; w < NW; ++w) {
-                                uint32_t x[4], y[4];
-                                e2m1x8_to_f16(lo[w], x);
-                                e2m1x8_to_f16(hi[w], y);
-                                const uint4 c4 = sm.turn[i][(4 * w + t) ^ swap], s4 = sm.turn[i][(4 * (NW + w) + t) ^ swap];
-                                const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint32_t xs = mul2(x[e], sl), ys = mul2(y[e], sh);
-                                    a_lo[r][4 * w + e] = fma2(neg2(ys), sn[e], mul2(xs, c[e]));
-                                    a_hi[r][4 * w + e] = fma2(xs, sn[e], mul2(ys, c[e]));
-                                }
-                            }
-                        }
-#pragma unroll
-                        for (int ks = 0; ks < 4 * NW; ++ks) {
-                            const uint32_t a[4] = {a_lo[0][ks], a_lo[1][ks], a_hi[0][ks], a_hi[1][ks]};
-                            mma_f16_16816(sc[j], a, qa[ks], qb[ks]);
-                        }
-                        const int left = n - (row0 + j * kUnit);
-                        if (left < kUnit) {                    // the request's last unit
-#pragma unroll
-                            for (int r = 0; r < 2; ++r)
-                                if (key_of(g + 8 * r) >= left) { sc[j][2 * r] = -INFINITY; sc[j][2 * r + 1] = -INFINITY; }
-                        }
-                        if (CAP) {
+                            const int key = key_of(g + 8 * r), swap = r * (D == 128 ? 4 : 2);      // r is the key's parity
+                            const unsigned char* row = st[j] + key * pitch + t * 4 * NW + 4 * w;
+                            const uint4* turn = sm.turn[(j == 0 ? in_macro : in_second) * kUnit + key];
+                            const uint4 c4 = turn[(4 * w + t) ^ swap], s4 = turn[(4 * (NW + w) + t) ^ swap];
+                            const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+                            uint32_t x[4], y[4];
+                            e2m1x8_to_f16(*reinterpret_cast<const uint32_t*>(row), x);
+                            e2m1x8_to_f16(*reinterpret_cast<const uint32_t*>(row + D / 4), y);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float x = sc[j][e] * ((e & 1) ? mul1 : mul0);
-                                sc[j][e] = x == -INFINITY ? x : p.logit_cap * tanhf(x / p.logit_cap) * kLog2e;
+                                const uint32_t xs = mul2(x[e], s_lo[j][r]), ys = mul2(y[e], s_hi[j][r]);
+                                a_lo[r][e] = fnma2(ys, sn[e], mul2(xs, c[e]));
+                                a_hi[r][e] = fma2(xs, sn[e], mul2(ys, c[e]));
                             }
                         }
-                    } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[j][e] = -INFINITY;
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t a[4] = {a_lo[0][e], a_lo[1][e], a_hi[0][e], a_hi[1][e]};
+                            mma_f16_16816(sc[j], a, qa[4 * w + e], qb[4 * w + e]);
+                        }
+                    }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int left = j < cnt ? n - (row0 + j * kUnit) : 0;
+                    if (left < kUnit) {                        // the request's last unit, or none
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            if (key_of(g + 8 * r) >= left) { sc[j][2 * r] = -INFINITY; sc[j][2 * r + 1] = -INFINITY; }
+                    }
+                    if (CAP) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = sc[j][e] * ((e & 1) ? mul1 : mul0);
+                            sc[j][e] = x == -INFINITY ? x : p.logit_cap * tanhf(x / p.logit_cap) * kLog2e;
+                        }
                     }
                 }
                 const float k0 = CAP ? 1.f : mul0, k1 = CAP ? 1.f : mul1;
@@ -532,17 +635,16 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                     l0 += pe[0] + pe[2];
                     l1 += pe[1] + pe[3];
                     const uint32_t b0 = transpose8(pack2(pe[0], pe[1])), b1 = transpose8(pack2(pe[2], pe[3]));
-                    const unsigned char* st = ring + (j == 0 ? stage : stage1) * (kUnit * Row::kBytes);
-                    const unsigned char* ra = st + key_of(2 * t) * Row::kBytes;           // keys of the fragment's columns 2t, 2t+1,
-                    const unsigned char* rb = st + key_of(2 * t + 1) * Row::kBytes;       // and one row further on 2t+8, 2t+9
+                    const unsigned char* ra = st[j] + key_of(2 * t) * pitch;           // keys of the fragment's columns 2t, 2t+1,
+                    const unsigned char* rb = st[j] + key_of(2 * t + 1) * pitch;       // and one row further on 2t+8, 2t+9
                     const int blk = g * (D / 8) / kQuantBlock;
                     uint32_t a[2][MT], h[2][MT];               // even and odd d of the thread's block; keys (2t, 2t+1), (2t+8, 2t+9)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         uint32_t wa[NW], wb[NW];
-                        load_words<D>(ra + r * Row::kBytes + Row::kV + g * 4 * NW, wa);
-                        load_words<D>(rb + r * Row::kBytes + Row::kV + g * 4 * NW, wb);
-                        const uint32_t s2 = e4m3x2_to_f16(ra[r * Row::kBytes + Row::kVScales + blk] | (uint32_t)rb[r * Row::kBytes + Row::kVScales + blk] << 8);
+                        load_words<D>(ra + r * pitch + Row::kV + g * 4 * NW, wa);
+                        load_words<D>(rb + r * pitch + Row::kV + g * 4 * NW, wb);
+                        const uint32_t s2 = e4m3x2_to_f16(ra[r * pitch + Row::kVScales + blk] | (uint32_t)rb[r * pitch + Row::kVScales + blk] << 8);
 #pragma unroll
                         for (int w = 0; w < NW; ++w) {
                             uint32_t x[4], y[4];
@@ -558,38 +660,38 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                         mma_f16_16816(o[i], f, b0, b1);
                     }
                 }
-                __syncwarp();                                  // every lane has read the stages that are requested into next
-                request(stage, next_a);
-                if (cnt == 2) {
-                    request(stage1, next_b);
-                    next_a = row_ids(s + kQtStages + 2);
-                    next_b = row_ids(s + kQtStages + 3);
-                    stage = stage1 + 1 == kQtStages ? 0 : stage1 + 1;
-                } else {
-                    next_a = next_b;
-                    next_b = row_ids(s + kQtStages + 2);
-                    stage = stage1;
+                __syncwarp();                                  // every lane has read the stages
+                if (lane == 0) {
+                    mbar_arrive(empty + 8 * stage);
+                    if (cnt == 2) mbar_arrive(empty + 8 * stage1);
                 }
+                if (cnt == 2) {
+                    stage = stage1;
+                    phase ^= stage1 == 0;
+                }
+                if (++stage == stages) { stage = 0; phase ^= 1; }
                 s += cnt;
                 in_macro += cnt;
-                if (in_macro == per) in_macro = 0;
+                unit += cnt;
+                if (in_macro == per) { in_macro = 0; unit += skip; }
             }
-            copies_wait<0>();
 #pragma unroll
             for (int off = 4; off <= 16; off <<= 1) {
                 l0 += __shfl_xor_sync(0xffffffffu, l0, off);
                 l1 += __shfl_xor_sync(0xffffffffu, l1, off);
             }
         }
-        // join the warps of a head; the ring is free
-        __syncwarp();
-        float* mine = reinterpret_cast<float*>(ring);          // [8][D]
+        // join the warps of a head; the rings are free
+        __syncthreads();
+        if (busy) {
+            float* mine = reinterpret_cast<float*>(rings) + warp * 8 * D;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            *reinterpret_cast<float2*>(mine + (2 * t) * D + g * (D / 8) + 2 * i) = make_float2(o[i][0], o[i][2]);
-            *reinterpret_cast<float2*>(mine + (2 * t + 1) * D + g * (D / 8) + 2 * i) = make_float2(o[i][1], o[i][3]);
+            for (int i = 0; i < MT; ++i) {
+                *reinterpret_cast<float2*>(mine + (2 * t) * D + g * (D / 8) + 2 * i) = make_float2(o[i][0], o[i][2]);
+                *reinterpret_cast<float2*>(mine + (2 * t + 1) * D + g * (D / 8) + 2 * i) = make_float2(o[i][1], o[i][3]);
+            }
         }
-        if (g == 0) { sm.ml[warp][2 * t] = make_float2(m0, l0); sm.ml[warp][2 * t + 1] = make_float2(m1, l1); }
+        if (busy && g == 0) { sm.ml[warp][2 * t] = make_float2(m0, l0); sm.ml[warp][2 * t + 1] = make_float2(m1, l1); }
         __syncthreads();
         if (busy) {
             const long long slot = blockIdx.x + b;
@@ -601,7 +703,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 for (int w = 0; w < share; ++w) {
                     const float2 ml = sm.ml[w * hpc + my_head][h];
                     const float weight = exp2_fast(ml.x - mm);
-                    sum += reinterpret_cast<const float*>(sm.ring[w * hpc + my_head][0])[h * D + d] * weight;
+                    sum += reinterpret_cast<const float*>(rings)[(w * hpc + my_head) * 8 * D + h * D + d] * weight;
                     l += ml.y * weight;
                 }
                 const long long at = slot * p.hq + kv * p.group + h;
@@ -609,9 +711,15 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 if (d == 0) p.part_ml[at] = make_float2(mm, l);
             }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next rows come behind the reads above
         __syncthreads();
         u0 = u1;
     }
+    if (requests && __any_sync(0xffffffffu, dead) && lane < share)       // given up: the copies still have to land (or time out)
+        for (int i = max(before - stages, 0); i < before; ++i) {
+            bool gone = false;
+            wait_phase(smem_u32(&sm.full[lane][i % stages]), i / stages & 1, p.status, gone);
+        }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -693,7 +801,7 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
     }
 }
 
-// Pieces the sequence of units is cut into: for the tensor cores one CTA per SM, sixteen warps over at most sixteen KV heads
+// Pieces the sequence of units is cut into: for the tensor cores one CTA per SM, eight warps over at most eight KV heads
 // each; for the CUDA cores what fits an SM.
 int tc_head_blocks(int hkv) { return (hkv + kQtWarps - 1) / kQtWarps; }
 int attend_pieces(int dtype, int hkv, int sms) {
@@ -709,14 +817,22 @@ cudaError_t launch_attend_plain(const QuantAttendParams& p, cudaStream_t stream)
     if (e != cudaSuccess) return e;
     return launch_chained(quant_merge_kernel<float, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
 }
-template <int D, bool CAP>
+template <int D, bool CAP, int PIECE>
 cudaError_t launch_attend_tc(const QuantAttendParams& p, cudaStream_t stream) {
     static SmemConfig configured = {};
-    cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP>, sizeof(QuantTcSmem<D>), configured);
+    cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP, PIECE>, kQtBytes, configured);
     if (e != cudaSuccess) return e;
-    e = launch_chained(quant_attend_tc_kernel<D, CAP>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), sizeof(QuantTcSmem<D>), stream, p);
+    e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), kQtBytes, stream, p);
     if (e != cudaSuccess) return e;
     return launch_chained(quant_merge_kernel<__nv_bfloat16, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+}
+template <int D, bool CAP>
+cudaError_t launch_attend_bf16(const QuantAttendParams& p, cudaStream_t stream) {
+    // Bulk copies and 16-byte pieces need rows, and a CTA's heads in them, that start on multiples of 16 bytes.
+    const int hpc = (p.hkv + tc_head_blocks(p.hkv) - 1) / tc_head_blocks(p.hkv);
+    const bool grid16 = p.hkv * QuantRow<D>::kBytes % 16 == 0 && (hpc == p.hkv || hpc * QuantRow<D>::kBytes % 16 == 0);
+    if (!grid16) return launch_attend_tc<D, CAP, 8>(p, stream);
+    return hpc * QuantRow<D>::kBytes < kQtBulkBytes ? launch_attend_tc<D, CAP, 16>(p, stream) : launch_attend_tc<D, CAP, 0>(p, stream);
 }
 
 }  // namespace
@@ -764,9 +880,8 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;
-    const bool cap = a->logit_cap > 0.f;
     if (a->dtype == TS_DTYPE_F32) e = a->head_dim == 128 ? launch_attend_plain<128>(p, s) : launch_attend_plain<64>(p, s);
-    else if (a->head_dim == 128) e = cap ? launch_attend_tc<128, true>(p, s) : launch_attend_tc<128, false>(p, s);
-    else e = cap ? launch_attend_tc<64, true>(p, s) : launch_attend_tc<64, false>(p, s);
+    else if (a->head_dim == 128) e = a->logit_cap > 0.f ? launch_attend_bf16<128, true>(p, s) : launch_attend_bf16<128, false>(p, s);
+    else e = a->logit_cap > 0.f ? launch_attend_bf16<64, true>(p, s) : launch_attend_bf16<64, false>(p, s);
     return e == cudaSuccess ? TS_OK : TS_ERR_CUDA;
 }
