@@ -1,8 +1,10 @@
 // ts_prompt_attend: causal attention of packed prompts, grouped heads.
 //
 //   o_i = sum_{j <= i, same sequence} softmax_j(cap(scale q_i . k_j)) v_j
-#include "ptx.cuh"
+#include <limits.h>
+
 #include "rope.cuh"
+#include "umma.cuh"
 
 namespace ts {
 namespace {
@@ -193,6 +195,426 @@ __global__ void __launch_bounds__(kPpThreads) prompt_plain_kernel(const PromptPa
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Tensor cores: bf16
+// ------------------------------------------------------------------------------------------------
+// A CTA takes tiles of 256 query tokens of one head as two halves of 128 rows, keys in blocks of 128:
+//   S_h (128 x 128 fp32)  = Q_h (shared memory, K-major) . K_b^T (shared memory, K-major)
+//   O_h (128 x D fp32)   += P_h (tensor memory, packed bf16, in the place of S_h) . V_b (shared memory, MN-major)
+// with S_0, S_1, O_0, O_1 in the 512 columns of tensor memory.  One thread issues every product, in the order
+//   P.V of half 0, Q.K^T of half 0 for the next block, P.V of half 1, Q.K^T of half 1 for the next block, ...
+// so the tensor pipe works on one half while 128 threads (one per row, so the row's maximum and sum need no exchange) turn
+// the other half's S into P.  A half's Q.K^T may overwrite its P because the products of one thread run in order, and S
+// complete means that every earlier P.V is: so those 128 threads also rescale O themselves, which they do only when a row's
+// maximum has grown by more than 2^8 since its reference was taken (P stays below 256).
+// One thread requests tiles (tiled copies, 128-byte swizzle): Q, and K and V blocks through a ring of five.  It runs ahead
+// into the CTA's next tile, of which it leaves the place in a two-entry queue.  Tiles are dealt out in the order of their
+// last key, longest first, heads innermost (the heads that share K and V run side by side).
+//
+// What is not finite.  A masked weight is 0, but 0 times an infinity in V is not; the block on the diagonal holds the V of
+// later tokens, and of the next sequence.  Only then does a row of O end up non-finite without cause, so rows that do are
+// computed again on the CUDA cores, from the keys that they see (slow, and exact for what is non-finite with cause).
+constexpr int kPtRows = 128, kPtBlock = 128;                   // rows of a half, keys of a block
+constexpr int kPtStages = 5, kPtThreads = 320;                 // two times four softmax warps, one that issues products, one that requests tiles
+constexpr int kPtQueue = 2;
+
+template <int D>
+struct PromptTcSmem {
+    unsigned char q[2][kPtRows * D * 2];                       // per half: D/64 parts of [128 rows][128 bytes]
+    unsigned char kv[kPtStages][kPtBlock * D * 2];
+    int4 queue[kPtQueue];                                      // first token, length, tile, head; length -1: no more
+    uint64_t q_full, q_empty, kv_full[kPtStages], kv_empty[kPtStages], s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint64_t queue_full[kPtQueue], queue_empty[kPtQueue], drained;
+    uint32_t tmem;
+};
+
+// Blocks of keys that half h of a tile sees; 0 when the sequence ends before it.
+__device__ __forceinline__ int blocks_of(int len, int tile, int h) {
+    const int row0 = tile * 2 * kPtRows + h * kPtRows;
+    return row0 < len ? min(row0 + kPtRows - 1, len - 1) / kPtBlock + 1 : 0;
+}
+
+// The warp that deals out tiles: positions 0, 1, ... name (sequence, tile) pairs by falling tile number, sequences in order
+// within one.
+struct TileOrder {
+    int level, from;                                           // tiles of this number start at position `from`
+};
+__device__ __forceinline__ int tiles_of(const PromptParams& p, int b) { return b < p.batch ? (sequence_of(p, b).y + 2 * kPtRows - 1) / (2 * kPtRows) : 0; }
+__device__ int count_tiles(const PromptParams& p, int above) {     // sequences with more tiles than `above`; all lanes call
+    int n = 0;
+    for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += tiles_of(p, b) > above;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+    return n;
+}
+// Sequence at place `rank` among those with more tiles than `level`.
+__device__ int sequence_at(const PromptParams& p, int level, int rank) {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < p.batch; base += 32) {
+        const unsigned has = __ballot_sync(0xffffffffu, tiles_of(p, base + lane) > level);
+        const int n = __popc(has);
+        if (rank < n) return base + __fns(has, 0, rank + 1);
+        rank -= n;
+    }
+    return 0;
+}
+
+// Row `row` of a sequence for one head on the CUDA cores, a warp per row: for rows that met what is not finite.
+template <int D>
+__device__ __noinline__ void prompt_row(const PromptParams& p, int first, int row, int h) {
+    const int lane = threadIdx.x & 31;
+    constexpr int E = D / 32;
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (long long)(first + row) * p.q_stride + (long long)h * D;
+    const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(p.k) + (long long)first * p.k_stride + (long long)(h / p.group) * D;
+    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v) + (long long)first * p.v_stride + (long long)(h / p.group) * D;
+    float x[E], o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) { x[e] = __bfloat162float(q[lane + 32 * e]); o[e] = 0.f; }
+    for (int j = 0; j <= row; ++j) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += x[e] * __bfloat162float(k[j * p.k_stride + lane + 32 * e]);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        s *= p.sm_scale;
+        if (p.logit_cap > 0.f) s = p.logit_cap * tanhf(s / p.logit_cap);
+        s *= 1.4426950408889634f;
+        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base), w = exp2f(s - base);
+        m = mn;
+        l = l * corr + w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * corr + w * __bfloat162float(v[j * p.v_stride + lane + 32 * e]);
+    }
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)(first + row) * p.hq + h) * D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CUtensorMap map_q,
+                                                                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    constexpr int kParts = D / 64;
+    constexpr uint32_t kPart = kPtRows * 128, kTile = kPart * kParts;      // bytes of 128 rows of 64 elements; of a tile
+    constexpr uint32_t kO = 256;                               // tensor memory: S_h at column 128 h, O_h at 256 + 128 h
+    extern __shared__ unsigned char dyn[];
+    PromptTcSmem<D>& sm = *reinterpret_cast<PromptTcSmem<D>*>(dyn + ((1024u - (smem_u32(dyn) & 1023u)) & 1023u));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&sm.q_full), 1);
+        mbar_init(smem_u32(&sm.q_empty), 1);
+        mbar_init(smem_u32(&sm.drained), 1);
+        for (int i = 0; i < kPtStages; ++i) { mbar_init(smem_u32(&sm.kv_full[i]), 1); mbar_init(smem_u32(&sm.kv_empty[i]), 1); }
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(smem_u32(&sm.s_full[h]), 1);
+            mbar_init(smem_u32(&sm.p_full[h]), 4);
+            mbar_init(smem_u32(&sm.o_full[h]), 1);
+            mbar_init(smem_u32(&sm.o_empty[h]), 4);
+        }
+        for (int i = 0; i < kPtQueue; ++i) { mbar_init(smem_u32(&sm.queue_full[i]), 1); mbar_init(smem_u32(&sm.queue_empty[i]), 9); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_before_sync();
+    __syncthreads();
+    tcgen05_after_sync();
+    const uint32_t tmem = *(volatile uint32_t*)&sm.tmem;
+    wait_for_predecessor();
+    bool dead = false;
+    // an entry of the queue; the last one says that there are no more
+    int taken = 0;
+    auto next_tile = [&]() {
+        const int i = taken % kPtQueue;
+        wait_phase(smem_u32(&sm.queue_full[i]), taken / kPtQueue & 1, p.status, dead);
+        dead = __any_sync(0xffffffffu, dead);                  // a warp gives up as one
+        const int4 t = dead ? make_int4(0, -1, 0, 0) : sm.queue[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.queue_empty[i]));
+        ++taken;
+        return t;
+    };
+
+    if (warp == 9) {
+        // ---------------- requests ----------------
+        TileOrder order = {0, 0};
+        {
+            int most = 0;
+            for (int b = lane; b < p.batch; b += 32) most = max(most, tiles_of(p, b));
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+            order.level = most - 1;
+        }
+        int here = order.level >= 0 ? count_tiles(p, order.level) : 0;     // tiles of this number
+        int kv = 0, put = 0;                                   // blocks requested, entries left so far
+        for (long long round = 0;; ++round, ++put) {
+            // items in snake order, so that a CTA's long and short ones balance
+            const long long item = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            const int pos = (int)min(item / p.hq, (long long)INT_MAX), head = (int)(item % p.hq);
+            while (order.level >= 0 && pos - order.from >= here) {
+                order.from += here;
+                --order.level;
+                here = order.level >= 0 ? count_tiles(p, order.level) : 0;
+            }
+            int4 t = make_int4(0, -1, 0, head);
+            if (order.level >= 0 && !dead) {
+                const int2 seq = sequence_of(p, sequence_at(p, order.level, pos - order.from));
+                t = make_int4(seq.x, seq.y, order.level, head);
+            }
+            const int i = put % kPtQueue;
+            wait_phase(smem_u32(&sm.queue_empty[i]), (put / kPtQueue & 1) ^ 1, p.status, dead);
+            dead = __any_sync(0xffffffffu, dead);
+            if (dead) t.y = -1;
+            __syncwarp();
+            if (lane == 0) { sm.queue[i] = t; mbar_arrive(smem_u32(&sm.queue_full[i])); }
+            if (t.y < 0) break;
+            const int n0 = blocks_of(t.y, t.z, 0), n1 = blocks_of(t.y, t.z, 1), n = max(n0, n1);
+            if (lane == 0) {
+                wait_phase(smem_u32(&sm.q_empty), (put & 1) ^ 1, p.status, dead);
+                mbar_expect_tx(smem_u32(&sm.q_full), n1 > 0 ? 2 * kTile : kTile);
+                for (int h = 0; h < (n1 > 0 ? 2 : 1); ++h)
+                    for (int c = 0; c < kParts; ++c)
+                        tile_g2s(smem_u32(sm.q[h]) + c * kPart, &map_q, 64 * c, t.w, t.x + t.z * 2 * kPtRows + h * kPtRows, smem_u32(&sm.q_full));
+                for (int j = 0; j < 2 * n; ++j, ++kv) {        // K_0, V_0, K_1, ...
+                    const int s = kv % kPtStages;
+                    wait_phase(smem_u32(&sm.kv_empty[s]), (kv / kPtStages & 1) ^ 1, p.status, dead);
+                    mbar_expect_tx(smem_u32(&sm.kv_full[s]), kTile);
+                    for (int c = 0; c < kParts; ++c)
+                        tile_g2s(smem_u32(sm.kv[s]) + c * kPart, j & 1 ? &map_v : &map_k, 64 * c, t.w / p.group, t.x + (j >> 1) * kPtBlock, smem_u32(&sm.kv_full[s]));
+                }
+            }
+            __syncwarp();
+            kv = __shfl_sync(0xffffffffu, kv, 0);
+        }
+        if (lane == 0 && dead) {                               // given up: the copies still have to land (or time out)
+            for (int i = max(kv - kPtStages, 0); i < kv; ++i) {
+                bool gone = false;
+                wait_phase(smem_u32(&sm.kv_full[i % kPtStages]), i / kPtStages & 1, p.status, gone);
+            }
+            bool gone = false;
+            if (put > 0) wait_phase(smem_u32(&sm.q_full), (put - 1) & 1, p.status, gone);
+        }
+        __syncwarp();
+    } else if (warp == 8) {
+        // ---------------- products ----------------
+        // instruction descriptors: fp32 accumulate, bf16 A and B, M = 128; N = 128 with K-major B, N = D with MN-major B
+        constexpr uint32_t kIdescQK = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+        int kv = 0, tiles = 0, p_count[2] = {0, 0}, o_count[2] = {0, 0};
+        for (;;) {
+            const int4 t = next_tile();
+            if (t.y < 0) break;
+            const int n_of[2] = {blocks_of(t.y, t.z, 0), blocks_of(t.y, t.z, 1)}, n = max(n_of[0], n_of[1]);
+            if (lane == 0) {
+                auto wait_block = [&](int i) {                 // block i of the tile's K_0, V_0, K_1, ...
+                    const int s = (kv + i) % kPtStages;
+                    wait_phase(smem_u32(&sm.kv_full[s]), (kv + i) / kPtStages & 1, p.status, dead);
+                    tcgen05_after_sync();
+                    return smem_u32(sm.kv[s]);
+                };
+                auto free_block = [&](int i) { mma_commit(smem_u32(&sm.kv_empty[(kv + i) % kPtStages])); };
+                auto issue_qk = [&](int h, uint32_t k) {
+                    const uint32_t q = smem_u32(sm.q[h]);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t off = (ks >> 2) * kPart + (ks & 3) * 32u;
+                        mma_ss(tmem + 128u * h, sw128_operand(q + off, 16, 1024), sw128_operand(k + off, 16, 1024), kIdescQK, ks > 0 ? 1u : 0u);
+                    }
+                    mma_commit(smem_u32(&sm.s_full[h]));
+                };
+                auto issue_pv = [&](int h, uint32_t v, bool first) {
+                    wait_phase(smem_u32(&sm.p_full[h]), p_count[h] & 1, p.status, dead);
+                    ++p_count[h];
+                    tcgen05_after_sync();
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)             // 16 keys a step: 8 columns of P
+                        mma_ts(tmem + kO + 128u * h, tmem + 128u * h + 8u * ks, sw128_operand(v + ks * 2048u, kPart, 1024), kIdescPV, !first || ks > 0 ? 1u : 0u);
+                };
+                wait_phase(smem_u32(&sm.q_full), tiles & 1, p.status, dead);
+                uint32_t k = wait_block(0);
+                issue_qk(0, k);
+                if (n_of[1] > 0) issue_qk(1, k);
+                free_block(0);
+                if (n == 1) mma_commit(smem_u32(&sm.q_empty));
+                for (int j = 0; j < n; ++j) {
+                    const uint32_t v = wait_block(2 * j + 1);
+                    k = j + 1 < n ? wait_block(2 * j + 2) : 0u;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (j < n_of[h]) {
+                            if (j == 0) {                      // the half's last result has been read
+                                wait_phase(smem_u32(&sm.o_empty[h]), (o_count[h] & 1) ^ 1, p.status, dead);
+                                ++o_count[h];
+                            }
+                            issue_pv(h, v, j == 0);
+                            if (j + 1 == n_of[h]) mma_commit(smem_u32(&sm.o_full[h]));
+                        }
+                        if (j + 1 < n_of[h]) issue_qk(h, k);
+                    }
+                    free_block(2 * j + 1);
+                    if (j + 1 < n) free_block(2 * j + 2);
+                    if (j + 2 == n) mma_commit(smem_u32(&sm.q_empty));
+                }
+            }
+            __syncwarp();
+            kv += 2 * n;
+            ++tiles;
+        }
+        if (lane == 0 && dead) {                               // given up: the products still have to end (or time out)
+            bool gone = false;
+            mma_commit(smem_u32(&sm.drained));
+            wait_phase(smem_u32(&sm.drained), 0, p.status, gone);
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax: half h, row r of it ----------------
+        const int h = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t at_s = tmem + ((uint32_t)(warp & 3) << 21) + 128u * h, at_o = at_s + kO;
+        const float cap = p.logit_cap, mul = CAP ? 1.f : p.sm_scale * 1.4426950408889634f;      // x * mul: base-2 units
+        int s_count = 0, o_count = 0;
+        for (;;) {
+            const int4 t = next_tile();
+            if (t.y < 0) break;
+            const int n = blocks_of(t.y, t.z, h);
+            if (n == 0) continue;
+            const int row = t.z * 2 * kPtRows + h * kPtRows + r;                  // in the sequence
+            float ref = 0.f, sum = 0.f;
+            for (int j = 0; j < n; ++j) {
+                wait_phase(smem_u32(&sm.s_full[h]), s_count & 1, p.status, dead);
+                ++s_count;
+                tcgen05_after_sync();
+                float x[kPtBlock];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_load32(at_s + 32u * c, x + 32 * c);
+                tmem_loads_done();
+                if (CAP) {
+#pragma unroll
+                    for (int c = 0; c < kPtBlock; ++c) x[c] = cap * tanhf(x[c] * p.sm_scale / cap) * 1.4426950408889634f;
+                }
+                if (j == n - 1) {                              // the diagonal; keys behind the sequence's end lie behind every row too
+                    const int lim = row - j * kPtBlock;
+#pragma unroll
+                    for (int c = 0; c < kPtBlock; ++c)
+                        if (c > lim) x[c] = -INFINITY;
+                }
+                float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int c = 4; c < kPtBlock; c += 4)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], x[c + i]);
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+                if (j == 0) {
+                    ref = fmaxf(mx, -1e30f);
+                } else if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
+                    const float corr = mx > ref + 8.f ? exp2f(ref - mx) : 1.f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        tmem_load32(at_o + 32u * c, o);
+                        tmem_loads_done();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= corr;
+                        tmem_store32(at_o + 32u * c, reinterpret_cast<const uint32_t*>(o));
+                    }
+                    sum *= corr;
+                    if (mx > ref + 8.f) ref = mx;
+                }
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float p0, p1;
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(fmaf(x[64 * c + 2 * e], mul, -ref)));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(fmaf(x[64 * c + 2 * e + 1], mul, -ref)));
+                        part[(2 * e) & 3] += p0;
+                        part[(2 * e + 1) & 3] += p1;
+                        w[e] = pack_bf16x2(p0, p1);
+                    }
+                    tmem_store32(at_s + 32u * c, w);
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_stores_done();
+                tcgen05_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[h]));
+            }
+            // the result
+            wait_phase(smem_u32(&sm.o_full[h]), o_count & 1, p.status, dead);
+            ++o_count;
+            tcgen05_after_sync();
+            const float inv = 1.f / sum;
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)(t.x + row) * p.hq + t.w) * D;
+            uint32_t top = 0;                                  // largest magnitude, NaN counting as the largest
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tmem_load32(at_o + 32u * c, o);
+                tmem_loads_done();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    o[e] *= inv;
+                    top = max(top, __float_as_uint(o[e]) & 0x7fffffffu);
+                }
+                if (row < t.y) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(pack_bf16x2(o[e], o[e + 1]), pack_bf16x2(o[e + 2], o[e + 3]),
+                                                                                 pack_bf16x2(o[e + 4], o[e + 5]), pack_bf16x2(o[e + 6], o[e + 7]));
+                }
+            }
+            tcgen05_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.o_empty[h]));
+            unsigned again = __ballot_sync(0xffffffffu, row < t.y && top >= 0x7f800000u);
+            for (; again != 0; again &= again - 1) prompt_row<D>(p, t.x, row - lane + __ffs(again) - 1, t.w);
+        }
+    }
+    tcgen05_before_sync();
+    __syncthreads();
+    if (warp == 8) {
+        tcgen05_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            ptr = nullptr;
+        return reinterpret_cast<EncodeTiled>(ptr);
+    }();
+    return f;
+}
+// [tokens][heads][D] bf16, boxes of 128 tokens x one head x 64 elements, 128-byte swizzle, zeros outside.
+bool tensor_map(CUtensorMap& m, const void* base, int d, int heads, int tokens, long long stride) {
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens}, strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, kPtBlock}, step[3] = {1, 1, 1};
+    return encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool CAP>
+cudaError_t launch_prompt_tc(const PromptParams& p, int sms, cudaStream_t stream) {
+    static SmemConfig configured = {};
+    constexpr size_t kSmem = sizeof(PromptTcSmem<D>) + 1024;
+    static_assert(kSmem <= 232448, "the kernel's shared memory must fit one CTA's maximum");
+    const cudaError_t e = ensure_dynamic_smem(prompt_tc_kernel<D, CAP>, kSmem, configured);
+    if (e != cudaSuccess) return e;
+    CUtensorMap q, k, v;
+    if (!encode_tiled() || !tensor_map(q, p.q, D, p.hq, p.tokens, p.q_stride) || !tensor_map(k, p.k, D, p.hkv, p.tokens, p.k_stride) ||
+        !tensor_map(v, p.v, D, p.hkv, p.tokens, p.v_stride))
+        return cudaErrorInvalidValue;
+    const long long items = ((long long)p.tokens / (2 * kPtRows) + p.batch) * p.hq;       // at most
+    return launch_chained(prompt_tc_kernel<D, CAP>, dim3((unsigned)(items < sms ? items : sms)), dim3(kPtThreads), kSmem, stream, p, q, k, v);
+}
+
 template <typename T, int D>
 cudaError_t launch_prompt_plain(const PromptParams& p, cudaStream_t stream) {
     static SmemConfig configured = {};
@@ -228,7 +650,11 @@ extern "C" int ts_prompt_attend(const ts_prompt_args* a) {
     p.sm_scale = a->sm_scale; p.logit_cap = a->logit_cap; p.status = a->status;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;
-    if (a->dtype == TS_DTYPE_BF16) e = a->head_dim == 128 ? launch_prompt_plain<__nv_bfloat16, 128>(p, s) : launch_prompt_plain<__nv_bfloat16, 64>(p, s);
-    else e = a->head_dim == 128 ? launch_prompt_plain<float, 128>(p, s) : launch_prompt_plain<float, 64>(p, s);
+    const int sms = sms_of(a->device);
+    if (sms <= 0) return TS_ERR_CUDA;
+    const bool cap = a->logit_cap > 0.f;
+    if (a->dtype == TS_DTYPE_F32) e = a->head_dim == 128 ? launch_prompt_plain<float, 128>(p, s) : launch_prompt_plain<float, 64>(p, s);
+    else if (a->head_dim == 128) e = cap ? launch_prompt_tc<128, true>(p, sms, s) : launch_prompt_tc<128, false>(p, sms, s);
+    else e = cap ? launch_prompt_tc<64, true>(p, sms, s) : launch_prompt_tc<64, false>(p, sms, s);
     return e == cudaSuccess ? TS_OK : TS_ERR_CUDA;
 }

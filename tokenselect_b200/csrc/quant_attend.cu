@@ -285,20 +285,6 @@ constexpr bool rings_fit() {
 }
 static_assert(rings_fit<128>() && rings_fit<64>(), "four stages for one warp of every head count");
 
-// Whether a phase is complete, without waiting for it (try_wait may suspend the warp for a while).
-__device__ __forceinline__ bool test_phase(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-// A wait of at most about a second; then the call's status says so, and the waits that follow give up at once.
-__device__ __forceinline__ void wait_phase(uint32_t bar, uint32_t parity, int* status, bool& dead) {
-    if (mbar_try_wait(bar, parity) || dead) return;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
-        if (clock64() - t0 > kWaitCycles) { report(status, TS_ERR_DEVICE_TIMEOUT); dead = true; return; }
-}
-
 // Key of a stage that M row m of a fragment stands for: rows 0..7 the even keys, 8..15 the odd ones, in an order in which
 // the four rows of a half-warp's read lie 32 bytes apart modulo 128, for K (rows g) and for V (rows 2t and 2t + 1) alike.
 __device__ __forceinline__ int key_of(int m) { return ((m & 4) ? 8 + (((m & 3) * 2) ^ 2) : (m & 3) * 2) + (m >> 3); }

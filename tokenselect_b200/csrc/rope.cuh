@@ -2,7 +2,7 @@
 #pragma once
 #include <math.h>
 
-#include "common.cuh"
+#include "ptx.cuh"
 
 namespace ts {
 
@@ -94,6 +94,20 @@ __device__ __forceinline__ void wait_for_predecessor() {
 
 __device__ __forceinline__ void report(int* status, int code) {
     if (status != nullptr) atomicCAS(status, 0, code);
+}
+
+// Whether a phase is complete, without waiting for it (try_wait may suspend the warp for a while).
+__device__ __forceinline__ bool test_phase(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A wait of at most about a second; then the call's status says so, and the waits that follow give up at once.
+__device__ __forceinline__ void wait_phase(uint32_t bar, uint32_t parity, int* status, bool& dead) {
+    if (mbar_try_wait(bar, parity) || dead) return;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (clock64() - t0 > kWaitCycles) { report(status, TS_ERR_DEVICE_TIMEOUT); dead = true; return; }
 }
 
 inline bool power_of_two(float g) {
