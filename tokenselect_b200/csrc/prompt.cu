@@ -205,8 +205,20 @@ __global__ void __launch_bounds__(kPpThreads) prompt_plain_kernel(const PromptPa
 //   P.V of half 0, Q.K^T of half 0 for the next block, P.V of half 1, Q.K^T of half 1 for the next block, ...
 // so the tensor pipe works on one half while 128 threads (one per row, so the row's maximum and sum need no exchange) turn
 // the other half's S into P.  A half's Q.K^T may overwrite its P because the products of one thread run in order, and S
-// complete means that every earlier P.V is: so those 128 threads also rescale O themselves, which they do only when a row's
-// maximum has grown by more than 2^8 since its reference was taken (P stays below 256).
+// complete means that every earlier P.V is: so those 128 threads also rescale O themselves.
+//
+// What bounds it, in this order as it was met (8192 tokens, 32 heads, 550 GFLOP):
+//  * the operands of the issuing thread.  Behind `lane == 0` each product's descriptors were moved into uniform registers
+//    anew, 80 cycles a product; behind elect.sync they are not (1091 -> 1190 TFLOP/s).
+//  * the way from S to P.  The weights of a block are taken with the reference that the blocks before left, 32 columns at a
+//    time as they arrive, instead of after the block's maximum: P in bf16 holds 2^127 as well as 1, so a maximum that grew
+//    is caught up with, by rescaling O and the sum, before the next block, and only when it grew by more than 2^8.  (A jump of
+//    more than 2^100 inside a block, which O might not hold, sends the row to the CUDA cores.)  P is handed over in two
+//    parts.  One pair of columns in four takes its exponentials on the multipliers: the exponential unit alone would need as
+//    long as the tensor pipe.  (1190 -> 1283; without the multipliers 1239, with one pair in three 1246, in eight 1230, P in
+//    one part 1218.)
+//  * now: power (1.59 GHz of 1.965 during the run); the tensor pipe is busy for 66 % of the cycles.
+//
 // One thread requests tiles (tiled copies, 128-byte swizzle): Q, and K and V blocks through a ring of five.  It runs ahead
 // into the CTA's next tile, of which it leaves the place in a two-entry queue.  Tiles are dealt out in the order of their
 // last key, longest first, heads innermost (the heads that share K and V run side by side).
@@ -223,7 +235,7 @@ struct PromptTcSmem {
     unsigned char q[2][kPtRows * D * 2];                       // per half: D/64 parts of [128 rows][128 bytes]
     unsigned char kv[kPtStages][kPtBlock * D * 2];
     int4 queue[kPtQueue];                                      // first token, length, tile, head; length -1: no more
-    uint64_t q_full, q_empty, kv_full[kPtStages], kv_empty[kPtStages], s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint64_t q_full, q_empty, kv_full[kPtStages], kv_empty[kPtStages], s_full[2], p_full[2][2], o_full[2], o_empty[2];
     uint64_t queue_full[kPtQueue], queue_empty[kPtQueue], drained;
     uint32_t tmem;
 };
@@ -290,6 +302,55 @@ __device__ __noinline__ void prompt_row(const PromptParams& p, int first, int ro
     for (int e = 0; e < E; ++e) out[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
 }
 
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x of two numbers on the multipliers, for x >= -125 (below, 2^-125): 2^n 2^f with n the nearest whole number and 2^f a
+// polynomial of degree 3 (Remez exchange: 7.5e-5 relative on [-1/2, 1/2], a twentieth of the weight's rounding to bf16).
+__device__ __forceinline__ uint64_t exp2_f32x2(uint64_t x) {
+    float a, b;
+    unpack_f32x2(x, a, b);
+    x = pack_f32x2(fmaxf(a, -125.f), fmaxf(b, -125.f));
+    const uint64_t magic = pack_f32x2(12582912.f, 12582912.f), minus = pack_f32x2(-12582912.f, -12582912.f);      // 1.5 * 2^23
+    const uint64_t n = add_f32x2(x, magic);                    // the nearest whole number in the lowest bits
+    const uint64_t f = fma_f32x2(add_f32x2(n, minus), pack_f32x2(-1.f, -1.f), x);
+    uint64_t y = fma_f32x2(f, pack_f32x2(0.0551716691f, 0.0551716691f), pack_f32x2(0.2426111222f, 0.2426111222f));
+    y = fma_f32x2(y, f, pack_f32x2(0.6932609855f, 0.6932609855f));
+    y = fma_f32x2(y, f, pack_f32x2(0.9999280735f, 0.9999280735f));
+    float ya, yb, na, nb;
+    unpack_f32x2(y, ya, yb);
+    unpack_f32x2(n, na, nb);
+    return pack_f32x2(__int_as_float(__float_as_int(ya) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(yb) + (__float_as_int(nb) << 23)));
+}
+template <bool B> struct Flag { static constexpr bool value = B; };
+
+// True for one lane of a converged warp.  (With `lane == 0` in its place the compiler does not know the code behind it to be
+// uniform and moves every operand of every product into uniform registers anew.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+
 template <int D, bool CAP>
 __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CUtensorMap map_q,
                                                                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -306,7 +367,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         for (int i = 0; i < kPtStages; ++i) { mbar_init(smem_u32(&sm.kv_full[i]), 1); mbar_init(smem_u32(&sm.kv_empty[i]), 1); }
         for (int h = 0; h < 2; ++h) {
             mbar_init(smem_u32(&sm.s_full[h]), 1);
-            mbar_init(smem_u32(&sm.p_full[h]), 4);
+            mbar_init(smem_u32(&sm.p_full[h][0]), 4);
+            mbar_init(smem_u32(&sm.p_full[h][1]), 4);
             mbar_init(smem_u32(&sm.o_full[h]), 1);
             mbar_init(smem_u32(&sm.o_empty[h]), 4);
         }
@@ -404,9 +466,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         int kv = 0, tiles = 0, p_count[2] = {0, 0}, o_count[2] = {0, 0};
         for (;;) {
             const int4 t = next_tile();
-            if (t.y < 0) break;
-            const int n_of[2] = {blocks_of(t.y, t.z, 0), blocks_of(t.y, t.z, 1)}, n = max(n_of[0], n_of[1]);
-            if (lane == 0) {
+            const int len = __shfl_sync(0xffffffffu, t.y, 0), tile = __shfl_sync(0xffffffffu, t.z, 0);
+            if (len < 0) break;
+            const int n_of[2] = {blocks_of(len, tile, 0), blocks_of(len, tile, 1)}, n = max(n_of[0], n_of[1]);
+            if (elect_one()) {
                 auto wait_block = [&](int i) {                 // block i of the tile's K_0, V_0, K_1, ...
                     const int s = (kv + i) % kPtStages;
                     wait_phase(smem_u32(&sm.kv_full[s]), (kv + i) / kPtStages & 1, p.status, dead);
@@ -424,12 +487,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     mma_commit(smem_u32(&sm.s_full[h]));
                 };
                 auto issue_pv = [&](int h, uint32_t v, bool first) {
-                    wait_phase(smem_u32(&sm.p_full[h]), p_count[h] & 1, p.status, dead);
-                    ++p_count[h];
-                    tcgen05_after_sync();
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)             // 16 keys a step: 8 columns of P
+                    for (int ks = 0; ks < 8; ++ks) {           // 16 keys a step: 8 columns of P, which comes in two parts
+                        if (ks % 4 == 0) {
+                            wait_phase(smem_u32(&sm.p_full[h][ks / 4]), p_count[h] & 1, p.status, dead);
+                            tcgen05_after_sync();
+                        }
                         mma_ts(tmem + kO + 128u * h, tmem + 128u * h + 8u * ks, sw128_operand(v + ks * 2048u, kPart, 1024), kIdescPV, !first || ks > 0 ? 1u : 0u);
+                    }
+                    ++p_count[h];
                 };
                 wait_phase(smem_u32(&sm.q_full), tiles & 1, p.status, dead);
                 uint32_t k = wait_block(0);
@@ -439,7 +505,6 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 if (n == 1) mma_commit(smem_u32(&sm.q_empty));
                 for (int j = 0; j < n; ++j) {
                     const uint32_t v = wait_block(2 * j + 1);
-                    k = j + 1 < n ? wait_block(2 * j + 2) : 0u;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (j < n_of[h]) {
@@ -450,7 +515,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                             issue_pv(h, v, j == 0);
                             if (j + 1 == n_of[h]) mma_commit(smem_u32(&sm.o_full[h]));
                         }
-                        if (j + 1 < n_of[h]) issue_qk(h, k);
+                        if (j + 1 < n_of[h]) issue_qk(h, wait_block(2 * j + 2));
                     }
                     free_block(2 * j + 1);
                     if (j + 1 < n) free_block(2 * j + 2);
@@ -479,35 +544,74 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             const int n = blocks_of(t.y, t.z, h);
             if (n == 0) continue;
             const int row = t.z * 2 * kPtRows + h * kPtRows + r;                  // in the sequence
-            float ref = 0.f, sum = 0.f;
+            float ref = 0.f, top_x = 0.f;                      // the row's reference; its largest logit so far
+            uint64_t sums[2] = {0ull, 0ull};                   // relative to the reference
+            bool fresh = true;
+            auto block = [&](auto last) {
+                constexpr bool diagonal = decltype(last)::value;
+                float x[2][32];
+                tmem_load32(at_s, x[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float (&y32)[32] = x[c & 1];
+                    tmem_loads_done();
+                    if (c < 3) tmem_load32(at_s + 32u * (c + 1), x[(c + 1) & 1]);
+                    if (CAP) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y32[e] = cap * tanhf(y32[e] * p.sm_scale / cap) * 1.4426950408889634f;
+                    }
+                    if (diagonal) {                            // the last block; keys behind the sequence's end lie behind every row too
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (32 * c + e > r) y32[e] = -INFINITY;
+                    }
+                    float m4[4] = {y32[0], y32[1], y32[2], y32[3]};
+#pragma unroll
+                    for (int e = 4; e < 32; e += 4)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], y32[e + i]);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+                    if (fresh) {                               // any number near the maximum will do: that of the first 32 keys
+                        ref = fmaxf(mx, -1e30f);
+                        top_x = ref;
+                        fresh = false;
+                    }
+                    top_x = fmaxf(top_x, mx);
+                    const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-ref, -ref);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint64_t y = fma_f32x2(pack_f32x2(y32[2 * e], y32[2 * e + 1]), mul2, ref2);
+                        float p0, p1;
+                        if (!diagonal && (e & 3) == 3) {       // (a masked weight has to be exactly 0)
+                            y = exp2_f32x2(y);
+                            unpack_f32x2(y, p0, p1);
+                        } else {
+                            unpack_f32x2(y, p0, p1);
+                            asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p0));
+                            asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(p1));
+                            y = pack_f32x2(p0, p1);
+                        }
+                        sums[e & 1] = add_f32x2(sums[e & 1], y);
+                        w[e] = pack_bf16x2(p0, p1);
+                    }
+                    tmem_store16(at_s + 16u * c, w);           // into columns that have been read
+                    if (c & 1) {
+                        tmem_stores_done();
+                        tcgen05_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[h][c >> 1]));
+                    }
+                }
+            };
             for (int j = 0; j < n; ++j) {
                 wait_phase(smem_u32(&sm.s_full[h]), s_count & 1, p.status, dead);
                 ++s_count;
                 tcgen05_after_sync();
-                float x[kPtBlock];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_load32(at_s + 32u * c, x + 32 * c);
-                tmem_loads_done();
-                if (CAP) {
-#pragma unroll
-                    for (int c = 0; c < kPtBlock; ++c) x[c] = cap * tanhf(x[c] * p.sm_scale / cap) * 1.4426950408889634f;
-                }
-                if (j == n - 1) {                              // the diagonal; keys behind the sequence's end lie behind every row too
-                    const int lim = row - j * kPtBlock;
-#pragma unroll
-                    for (int c = 0; c < kPtBlock; ++c)
-                        if (c > lim) x[c] = -INFINITY;
-                }
-                float m4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int c = 4; c < kPtBlock; c += 4)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], x[c + i]);
-                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
-                if (j == 0) {
-                    ref = fmaxf(mx, -1e30f);
-                } else if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
-                    const float corr = mx > ref + 8.f ? exp2f(ref - mx) : 1.f;
+                // The blocks before raised a row's maximum by more than 2^8: O (every P.V so far is complete) and the sum follow.
+                if (__any_sync(0xffffffffu, top_x > ref + 8.f)) {
+                    const bool grown = top_x > ref + 8.f;
+                    const float corr = grown ? exp2f(ref - top_x) : 1.f;
 #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
                         float o[32];
@@ -517,30 +621,19 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                         for (int e = 0; e < 32; ++e) o[e] *= corr;
                         tmem_store32(at_o + 32u * c, reinterpret_cast<const uint32_t*>(o));
                     }
-                    sum *= corr;
-                    if (mx > ref + 8.f) ref = mx;
+                    const uint64_t corr2 = pack_f32x2(corr, corr);
+                    sums[0] = mul_f32x2(sums[0], corr2);
+                    sums[1] = mul_f32x2(sums[1], corr2);
+                    // a jump that P, up to 2^127 in bf16, or O would not hold: the row is computed again at the end
+                    if (top_x > ref + 100.f) sums[0] = pack_f32x2(__int_as_float(0x7fc00000), 0.f);
+                    if (grown) ref = top_x;
                 }
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float p0, p1;
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(fmaf(x[64 * c + 2 * e], mul, -ref)));
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(fmaf(x[64 * c + 2 * e + 1], mul, -ref)));
-                        part[(2 * e) & 3] += p0;
-                        part[(2 * e + 1) & 3] += p1;
-                        w[e] = pack_bf16x2(p0, p1);
-                    }
-                    tmem_store32(at_s + 32u * c, w);
-                }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                tmem_stores_done();
-                tcgen05_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[h]));
+                if (j == n - 1) block(Flag<true>()); else block(Flag<false>());
             }
+            float sum, sum1;
+            unpack_f32x2(add_f32x2(sums[0], sums[1]), sum, sum1);
+            sum += sum1;
+            if (top_x > ref + 100.f) sum = __int_as_float(0x7fc00000);
             // the result
             wait_phase(smem_u32(&sm.o_full[h]), o_count & 1, p.status, dead);
             ++o_count;
