@@ -356,7 +356,7 @@ typedef struct ts_quant_rows_args {
     int32_t dtype;                 /* TS_DTYPE_* of k and v */
     int32_t hkv;                   /* KV heads, 1 .. 1024 */
     int32_t head_dim;              /* 64 or 128 */
-    int32_t count;                 /* rows; 0 does nothing */
+    int32_t count;                 /* rows; 0 does nothing; count*hkv*head_dim/8 < 2^32 - 256 (TS_ERR_CAPACITY otherwise) */
     void* k;                       /* row i, head h at k + i*k_stride + h*head_dim (elements); read by write, written by read */
     void* v;
     int64_t k_stride;              /* elements between rows, >= hkv*head_dim */

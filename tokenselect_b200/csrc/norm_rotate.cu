@@ -3,10 +3,11 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w,   (y_i, y_{i+D/2}) -> (y_i cos - y_{i+D/2} sin, y_{i+D/2} cos + y_i sin)
 //
 // What bounds it: HBM (a row is read once, written once, a key row twice) and, for a few tokens, the launch.  Eight lanes
-// hold one (token, head) row: lane l the elements [P l, P l + P) of both halves (P = D/16), that is both members of its
-// rotation pairs, so the rotation exchanges nothing and the norm three shuffles.  Each thread evaluates the D/16 angles it
-// needs itself: an integer product each (rope.cuh), and in bf16 the fast sine and cosine, whose 2^-20 is far below the
-// output's 2^-9.  No table, no shared memory, no barrier: a block's rows are independent.
+// hold the rows of up to four neighbouring heads of a token: lane l the elements [P l, P l + P) of both halves of each
+// (P = D/16), that is both members of its rotation pairs, so the rotation exchanges nothing and the norm three shuffles, and
+// the angles (an integer product each, rope.cuh, and in bf16 the fast sine and cosine, whose 2^-20 is far below the output's
+// 2^-9) are evaluated once for four heads.  All rows are requested before the first is used.  No table, no shared memory, no
+// barrier: the groups of eight lanes are independent.
 #include "ptx.cuh"
 #include "rope.cuh"
 
@@ -15,6 +16,7 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormLanes = 8;                                  // lanes a row
+constexpr int kNormHeads = 4;                                  // rows of a group of lanes
 
 struct NormParams {
     const void* q;
@@ -26,8 +28,9 @@ struct NormParams {
     void* q_out;
     void* k_out;
     void* k_plain;
-    int hq, heads;                                             // heads = hq + hkv
-    long long rows;                                            // tokens * heads
+    int hq, hkv;
+    unsigned groups_q, per_token;                              // groups of four heads: of the queries, of a token
+    unsigned long long groups;
     float eps;
     TurnFreqs freqs;
 };
@@ -74,53 +77,73 @@ template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_constant__ NormParams p) {
     constexpr int P = D / 2 / kNormLanes;
     const int lane = threadIdx.x % kNormLanes;
-    const long long row = (long long)blockIdx.x * (kNormThreads / kNormLanes) + threadIdx.x / kNormLanes;
-    const bool mine = row < p.rows;                            // the others keep their warp's shuffles company
-    const long long t = mine ? row / p.heads : 0;
-    const int h = mine ? (int)(row - t * p.heads) : 0;
-    const bool is_q = h < p.hq;
-    const int hh = is_q ? h : h - p.hq;
-    const T* src = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_stride : reinterpret_cast<const T*>(p.k) + t * p.k_stride) +
-                   (long long)hh * D + P * lane;
+    const unsigned long long group = (unsigned long long)blockIdx.x * (kNormThreads / kNormLanes) + threadIdx.x / kNormLanes;
+    const bool mine = group < p.groups;                        // the others keep their warp's shuffles company
+    const unsigned long long t64 = mine ? group / p.per_token : 0;
+    const long long t = (long long)t64;
+    const unsigned part = mine ? (unsigned)(group - t64 * p.per_token) : 0u;
+    const bool is_q = part < p.groups_q;
+    const int h0 = (int)(is_q ? part : part - p.groups_q) * kNormHeads, count = min(kNormHeads, (is_q ? p.hq : p.hkv) - h0);
+    const T* src = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_stride : reinterpret_cast<const T*>(p.k) + t * p.k_stride) + h0 * D + P * lane;
     const T* w = reinterpret_cast<const T*>(is_q ? p.q_weight : p.k_weight);
     wait_for_predecessor();
-    float lo[P], hi[P];
-    load_row<T, P, WIDE>(src, lo);
-    load_row<T, P, WIDE>(src + D / 2, hi);
+    float lo[kNormHeads][P], hi[kNormHeads][P];
+#pragma unroll
+    for (int i = 0; i < kNormHeads; ++i) {                     // behind the last head: that one again
+        load_row<T, P, WIDE>(src + min(i, count - 1) * D, lo[i]);
+        load_row<T, P, WIDE>(src + min(i, count - 1) * D + D / 2, hi[i]);
+    }
     if (p.q_weight != nullptr || p.k_weight != nullptr) {      // uniform: whether any row of the launch is normed
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < P; ++e) sum += lo[e] * lo[e] + hi[e] * hi[e];
-#pragma unroll
-        for (int off = 1; off < kNormLanes; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        float a[P], b[P];
         if (w != nullptr) {
-            const float r = rsqrtf(sum * (1.f / D) + p.eps);
-            float a[P], b[P];
             load_row<T, P, WIDE>(w + P * lane, a);
             load_row<T, P, WIDE>(w + D / 2 + P * lane, b);
+        }
 #pragma unroll
-            for (int e = 0; e < P; ++e) { lo[e] = lo[e] * r * a[e]; hi[e] = hi[e] * r * b[e]; }
+        for (int i = 0; i < kNormHeads; ++i) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < P; ++e) sum += lo[i][e] * lo[i][e] + hi[i][e] * hi[i][e];
+#pragma unroll
+            for (int off = 1; off < kNormLanes; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if (w != nullptr) {
+                const float r = rsqrtf(sum * (1.f / D) + p.eps);
+#pragma unroll
+                for (int e = 0; e < P; ++e) { lo[i][e] = lo[i][e] * r * a[e]; hi[i][e] = hi[i][e] * r * b[e]; }
+            }
         }
     }
     if (!mine) return;
-    const long long at = (is_q ? t * p.hq + hh : t * (p.heads - p.hq) + hh) * D + P * lane;
+    const long long at = (t * (is_q ? p.hq : p.hkv) + h0) * D + P * lane;
     if (!is_q && p.k_plain != nullptr) {
-        store_row<T, P, WIDE>(reinterpret_cast<T*>(p.k_plain) + at, lo);
-        store_row<T, P, WIDE>(reinterpret_cast<T*>(p.k_plain) + at + D / 2, hi);
+        T* plain = reinterpret_cast<T*>(p.k_plain) + at;
+#pragma unroll
+        for (int i = 0; i < kNormHeads; ++i)
+            if (i < count) {
+                store_row<T, P, WIDE>(plain + i * D, lo[i]);
+                store_row<T, P, WIDE>(plain + i * D + D / 2, hi[i]);
+            }
     }
     if (p.positions != nullptr) {
         const long long pos = p.positions[t];
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             const float2 cs = sizeof(T) == 2 ? cos_sin_fast(pos, p.freqs.f[P * lane + e]) : cos_sin(pos, p.freqs.f[P * lane + e]);
-            const float x = lo[e], y = hi[e];
-            lo[e] = x * cs.x - y * cs.y;
-            hi[e] = y * cs.x + x * cs.y;
+#pragma unroll
+            for (int i = 0; i < kNormHeads; ++i) {
+                const float x = lo[i][e], y = hi[i][e];
+                lo[i][e] = x * cs.x - y * cs.y;
+                hi[i][e] = y * cs.x + x * cs.y;
+            }
         }
     }
     T* out = reinterpret_cast<T*>(is_q ? p.q_out : p.k_out) + at;
-    store_row<T, P, WIDE>(out, lo);
-    store_row<T, P, WIDE>(out + D / 2, hi);
+#pragma unroll
+    for (int i = 0; i < kNormHeads; ++i)
+        if (i < count) {
+            store_row<T, P, WIDE>(out + i * D, lo[i]);
+            store_row<T, P, WIDE>(out + i * D + D / 2, hi[i]);
+        }
 }
 
 template <typename T, int D>
@@ -129,7 +152,7 @@ cudaError_t launch_norm_rotate(const NormParams& p, cudaStream_t stream) {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.q_weight) |
                            reinterpret_cast<uintptr_t>(p.k_weight) | reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out) |
                            reinterpret_cast<uintptr_t>(p.k_plain) | (uintptr_t)(p.q_stride * sizeof(T)) | (uintptr_t)(p.k_stride * sizeof(T));
-    const dim3 grid((unsigned)((p.rows * kNormLanes + kNormThreads - 1) / kNormThreads));
+    const dim3 grid((unsigned)((p.groups * kNormLanes + kNormThreads - 1) / kNormThreads));
     return bits % kAlign == 0 ? launch_chained(norm_rotate_kernel<T, D, true>, grid, dim3(kNormThreads), 0, stream, p)
                               : launch_chained(norm_rotate_kernel<T, D, false>, grid, dim3(kNormThreads), 0, stream, p);
 }
@@ -154,8 +177,11 @@ extern "C" int ts_norm_rotate(const ts_norm_rotate_args* a) {
     p.q = a->q; p.k = a->k; p.q_stride = a->q_stride; p.k_stride = a->k_stride;
     p.positions = a->positions; p.q_weight = a->q_weight; p.k_weight = a->k_weight;
     p.q_out = a->q_out; p.k_out = a->k_out; p.k_plain = a->k_plain;
-    p.hq = a->hq; p.heads = a->hq + a->hkv; p.rows = (long long)a->tokens * p.heads; p.eps = a->eps;
-    if (p.rows > (1ll << 31) * (kNormThreads / kNormLanes) - kNormThreads) return TS_ERR_INVALID_ARG;      // blocks of one launch
+    p.hq = a->hq; p.hkv = a->hkv; p.eps = a->eps;
+    p.groups_q = (a->hq + kNormHeads - 1) / kNormHeads;
+    p.per_token = p.groups_q + (a->hkv + kNormHeads - 1) / kNormHeads;
+    p.groups = (unsigned long long)a->tokens * p.per_token;
+    if (p.groups > ((1ull << 31) - 1) * (kNormThreads / kNormLanes)) return TS_ERR_CAPACITY;      // blocks of one launch
     if (a->positions) p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;

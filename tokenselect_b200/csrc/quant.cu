@@ -25,7 +25,7 @@ struct QuantRowsParams {
     const int* rows;
     unsigned char* pool;
     long long pool_rows;
-    long long blocks;                                          // count * hkv * 2 * head_dim/16
+    unsigned blocks;                                           // count * hkv * 2 * head_dim/16
     int hkv;
     float k_scale, v_scale;
     int* status;
@@ -55,26 +55,36 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&x)[kQuantBlock]
     for (int e = 0; e < kQuantBlock; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     w = make_uint2(0u, 0u);
     if (top >= 0x7f800000u) return 0x7fu;                      // an infinity or a NaN: the scale is NaN
-    const float inv_g = 1.f / g;
-    const uint32_t scale = f32_to_e4m3(fminf(__fdiv_rn(__uint_as_float(top) * inv_g, 6.f), 448.f));
+    const float inv_g = 1.f / g, most = __uint_as_float(top) * inv_g;
+    const uint32_t scale = f32_to_e4m3(fminf(__fdiv_rn(most, 6.f), 448.f));
     if (scale == 0) return 0;
     const float s = e4m3_to_f32(scale);
     float y[2][8];
+    if (most < 1e30f) {
+        // Sixteen quotients by one divisor: Markstein's correction (1990) of the product with the rounded reciprocal gives the
+        // rounded quotient in three operations.
+        const float inv_s = __fdiv_rn(1.f, s);
 #pragma unroll
-    for (int e = 0; e < kQuantBlock; ++e) y[e >> 3][e & 7] = __fdiv_rn(x[e] * inv_g, s);
+        for (int e = 0; e < kQuantBlock; ++e) {
+            const float v = x[e] * inv_g, q = v * inv_s;
+            y[e >> 3][e & 7] = fmaf(fmaf(-q, s, v), inv_s, q);
+        }
+    } else {                                                   // far beyond what the scale can hold, where v may be infinite
+#pragma unroll
+        for (int e = 0; e < kQuantBlock; ++e) y[e >> 3][e & 7] = __fdiv_rn(x[e] * inv_g, s);
+    }
     w = make_uint2(f32x8_to_e2m1(y[0]), f32x8_to_e2m1(y[1]));
     return scale;
 }
 
 struct BlockPlace { int i, head, part; bool is_v; };           // row of the call, head, block of the head
 template <int D>
-__device__ __forceinline__ BlockPlace block_place(long long b, int hkv) {
-    constexpr int kParts = D / kQuantBlock;
+__device__ __forceinline__ BlockPlace block_place(unsigned b, unsigned hkv) {
+    constexpr unsigned kParts = D / kQuantBlock;
     BlockPlace r;
     r.part = (int)(b % kParts);
-    const long long u = b / kParts;                            // (row, K or V, head)
-    r.head = (int)(u % hkv);
-    const long long w = u / hkv;
+    const unsigned u = b / kParts, w = u / hkv;                // (row, K or V, head)
+    r.head = (int)(u - w * hkv);
     r.is_v = (w & 1) != 0;
     r.i = (int)(w >> 1);
     return r;
@@ -83,7 +93,7 @@ __device__ __forceinline__ BlockPlace block_place(long long b, int hkv) {
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads) quant_write_kernel(const QuantRowsParams p) {
     using Row = QuantRow<D>;
-    const long long b = (long long)blockIdx.x * kRowsThreads + threadIdx.x;
+    const unsigned b = blockIdx.x * kRowsThreads + threadIdx.x;
     wait_for_predecessor();
     if (b >= p.blocks) return;
     const BlockPlace at = block_place<D>(b, p.hkv);
@@ -102,7 +112,7 @@ __global__ void __launch_bounds__(kRowsThreads) quant_write_kernel(const QuantRo
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads) quant_read_kernel(const QuantRowsParams p) {
     using Row = QuantRow<D>;
-    const long long b = (long long)blockIdx.x * kRowsThreads + threadIdx.x;
+    const unsigned b = blockIdx.x * kRowsThreads + threadIdx.x;
     wait_for_predecessor();
     if (b >= p.blocks) return;
     const BlockPlace at = block_place<D>(b, p.hkv);
@@ -164,8 +174,9 @@ int quant_rows(const ts_quant_rows_args* a, bool write) {
     QuantRowsParams p;
     p.k = a->k; p.v = a->v; p.k_stride = a->k_stride; p.v_stride = a->v_stride; p.rows = a->rows;
     p.pool = static_cast<unsigned char*>(a->pool); p.pool_rows = a->pool_rows; p.hkv = a->hkv;
-    p.blocks = (long long)a->count * a->hkv * 2 * (a->head_dim / kQuantBlock);
-    if (p.blocks > ((1ll << 31) - 1) * kRowsThreads) return TS_ERR_INVALID_ARG;
+    const long long blocks = (long long)a->count * a->hkv * 2 * (a->head_dim / kQuantBlock);
+    if (blocks >= (1ll << 32) - kRowsThreads) return TS_ERR_CAPACITY;         // blocks are counted in 32 bits
+    p.blocks = (unsigned)blocks;
     p.k_scale = a->k_scale; p.v_scale = a->v_scale; p.status = a->status;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;

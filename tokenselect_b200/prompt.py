@@ -16,26 +16,30 @@ from ._lib import TsNormRotateArgs, TsPromptArgs, check
 from .engine import _raw_stream
 
 _NORM_ARGS_SIZE, _PROMPT_ARGS_SIZE = C.sizeof(TsNormRotateArgs), C.sizeof(TsPromptArgs)
+_lib_ = _lib.load                # the library, loaded at the first call
 _DTYPES = {torch.bfloat16: _lib.TS_DTYPE_BF16, torch.float32: _lib.TS_DTYPE_F32}
 
 
-def _token_stride(name: str, t: torch.Tensor, like: torch.Tensor, device: int) -> int:
-    """Elements between the tokens of ``[tokens, heads, head_dim]``; raises unless the heads of a token are packed."""
-    if t.dim() != 3 or t.get_device() != device or device < 0 or t.dtype != like.dtype or t.dtype not in _DTYPES \
-            or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]:
+def _token_stride(name: str, t: torch.Tensor, n: int, d: int, dtype: torch.dtype, device: int) -> int:
+    """Elements between the tokens of ``[n, heads, d]``; raises unless the heads of a token are packed."""
+    shape = t.shape
+    if len(shape) != 3 or t.get_device() != device or device < 0 or t.dtype != dtype or dtype not in _DTYPES or shape[0] != n \
+            or shape[2] != d:
         raise ValueError(f"{name} must be a CUDA tensor [tokens, heads, head_dim] in bf16 or fp32, all of one type and device")
-    n, heads, d = t.shape
-    s = t.stride()
-    if n == 0:
-        return heads * d
-    if s[2] != 1 or (heads > 1 and s[1] != d) or (n > 1 and s[0] < heads * d):
+    s0, s1, s2 = t.stride()
+    row = shape[1] * d
+    if n > 1 and s2 == 1 and s1 == d and s0 >= row:
+        return s0
+    if n > 0 and (s2 != 1 or (shape[1] > 1 and s1 != d) or (n > 1 and s0 < row)):
         raise ValueError(f"{name}: the heads of a token must follow each other without gaps, and tokens not overlap")
-    return s[0] if n > 1 else heads * d
+    return s0 if n > 1 else row
 
 
 def _check_out(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device or not t.is_contiguous():
+    if t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device() or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous, of its input's shape, type and device")
+    if t.data_ptr() == like.data_ptr() and not like.is_contiguous():
+        raise ValueError(f"{name} may be its input only where that is contiguous")
 
 
 def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tensor], rope_base: float = 1e6,
@@ -48,31 +52,39 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tens
     rounded once.  Returns ``(q, k)``, and behind them the normed keys before the rotation, for the cache, when
     ``with_plain_k`` or ``k_plain`` asks for them.  Inputs may be slices of a fused projection's output; outputs are
     contiguous, and may be the inputs themselves where those are."""
-    dev = q.get_device()
-    qs, ks = _token_stride("q", q, q, dev), _token_stride("k", k, q, dev)
-    n, hq, d = q.shape
+    # One token costs the device less than a generous host path costs Python: one look at each property.
+    dev, dtype, shape = q.get_device(), q.dtype, q.shape
+    if len(shape) != 3:
+        raise ValueError("q must be [tokens, heads, head_dim]")
+    n, hq, d = shape
+    qs, ks = _token_stride("q", q, n, d, dtype, dev), _token_stride("k", k, n, d, dtype, dev)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != q.dtype or w.get_device() != dev or w.shape != (d,) or not w.is_contiguous()):
+        if w is not None and (w.dtype != dtype or w.get_device() != dev or w.shape != (d,) or not w.is_contiguous()):
             raise ValueError(f"{name} must be [head_dim] of q's type on q's device")
     if positions is not None and (positions.dtype != torch.int32 or positions.get_device() != dev or positions.shape != (n,)
                                   or not positions.is_contiguous()):
         raise ValueError("positions must be a contiguous int32 tensor [tokens] on q's device")
-    outs = []
-    for name, t, like, wanted in (("q_out", q_out, q, True), ("k_out", k_out, k, True), ("k_plain", k_plain, k, with_plain_k)):
-        if t is not None:
-            _check_out(name, t, like)
-            if t.data_ptr() == like.data_ptr() and not like.is_contiguous():
-                raise ValueError(f"{name} may be its input only where that is contiguous")
-        elif wanted:
-            t = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-        if t is not None:
-            outs.append(t)
-    a = TsNormRotateArgs(_NORM_ARGS_SIZE, dev, _DTYPES[q.dtype], n, hq, k.shape[1], d, eps, q.data_ptr(), k.data_ptr(), qs, ks,
+    packed = torch.contiguous_format
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=packed)
+    else:
+        _check_out("q_out", q_out, q)
+    if k_out is None:
+        k_out = torch.empty_like(k, memory_format=packed)
+    else:
+        _check_out("k_out", k_out, k)
+    if k_plain is None:
+        k_plain = torch.empty_like(k, memory_format=packed) if with_plain_k else None
+    else:
+        _check_out("k_plain", k_plain, k)
+        if k_plain.data_ptr() == k_out.data_ptr() and n > 0:
+            raise ValueError("k_plain and k_out hold different results")
+    a = TsNormRotateArgs(_NORM_ARGS_SIZE, dev, _DTYPES[dtype], n, hq, k.shape[1], d, eps, q.data_ptr(), k.data_ptr(), qs, ks,
                          None if positions is None else positions.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
-                         None if k_weight is None else k_weight.data_ptr(), rope_base, rope_scale, outs[0].data_ptr(),
-                         outs[1].data_ptr(), outs[2].data_ptr() if len(outs) > 2 else None, _raw_stream(dev))
-    check(_lib.load().ts_norm_rotate(C.byref(a)), "ts_norm_rotate")
-    return tuple(outs)
+                         None if k_weight is None else k_weight.data_ptr(), rope_base, rope_scale, q_out.data_ptr(),
+                         k_out.data_ptr(), None if k_plain is None else k_plain.data_ptr(), _raw_stream(dev))
+    check(_lib_().ts_norm_rotate(C.byref(a)), "ts_norm_rotate")
+    return (q_out, k_out) if k_plain is None else (q_out, k_out, k_plain)
 
 
 def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, sm_scale: float,
@@ -83,9 +95,11 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens:
     head_dim]``; rows behind the last sequence are left as they were in ``out``.  The tensors start on 16 bytes and
     their tokens lie a multiple of 16 bytes apart (slices of a fused projection do).  ``status`` (optional, int32) is
     set when a bound of ``cu_seqlens`` makes no sense; the sequence then ends where it still does."""
-    dev = q.get_device()
-    qs, ks, vs = _token_stride("q", q, q, dev), _token_stride("k", k, q, dev), _token_stride("v", v, q, dev)
-    n, hq, d = q.shape
+    dev, dtype, shape = q.get_device(), q.dtype, q.shape
+    if len(shape) != 3:
+        raise ValueError("q must be [tokens, heads, head_dim]")
+    n, hq, d = shape
+    qs, ks, vs = (_token_stride(name, t, n, d, dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
     hkv = k.shape[1]
     if v.shape[1] != hkv or hkv == 0 or hq % hkv != 0:
         raise ValueError("k and v must have the same heads, a divisor of q's")
@@ -95,11 +109,11 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens:
     if status is not None and (status.dtype != torch.int32 or status.get_device() != dev):
         raise ValueError("status must be an int32 tensor on q's device")
     if out is None:
-        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_out("out", out, q)
-    a = TsPromptArgs(_PROMPT_ARGS_SIZE, dev, _DTYPES[q.dtype], n, cu_seqlens.numel() - 1, hq, hkv, d, sm_scale, logit_cap,
+    a = TsPromptArgs(_PROMPT_ARGS_SIZE, dev, _DTYPES[dtype], n, cu_seqlens.numel() - 1, hq, hkv, d, sm_scale, logit_cap,
                      q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, cu_seqlens.data_ptr(), out.data_ptr(),
                      None if status is None else status.data_ptr(), _raw_stream(dev))
-    check(_lib.load().ts_prompt_attend(C.byref(a)), "ts_prompt_attend")
+    check(_lib_().ts_prompt_attend(C.byref(a)), "ts_prompt_attend")
     return out

@@ -39,12 +39,17 @@ def kv4_pool(rows: int, num_kv_heads: int, head_dim: int, device="cuda") -> torc
     return torch.zeros((rows, num_kv_heads, kv4_row_bytes(head_dim)), dtype=torch.uint8, device=device)
 
 
+_HEAD_DIMS = {kv4_row_bytes(d): d for d in (64, 128)}
+_lib_ = _lib.load                # the library, loaded at the first call
+
+
 def _check_pool(pool: torch.Tensor) -> int:
     """The pool's head_dim."""
-    if pool.dim() != 3 or pool.dtype != torch.uint8 or not pool.is_cuda or not pool.is_contiguous() or pool.shape[0] == 0:
+    shape = pool.shape
+    if len(shape) != 3 or pool.dtype != torch.uint8 or not pool.is_cuda or not pool.is_contiguous() or shape[0] == 0:
         raise ValueError("pool must be a contiguous CUDA uint8 tensor [rows, num_kv_heads, 9*head_dim/8]")
-    d = pool.shape[2] * 8 // 9
-    if d not in (64, 128) or pool.shape[2] * 8 != d * 9:
+    d = _HEAD_DIMS.get(shape[2])
+    if d is None:
         raise ValueError("pool rows are 72 bytes a head (head_dim 64) or 144 (head_dim 128)")
     return d
 
@@ -55,17 +60,25 @@ def _check_ints(device: int, named) -> None:
             raise ValueError(f"{name} must be a contiguous int32 tensor on the pool's device")
 
 
-def _row_args(pool, k, v, rows, k_scale, v_scale, status) -> TsQuantRowsArgs:
-    d, dev, (pool_rows, heads, _) = _check_pool(pool), pool.get_device(), pool.shape
-    n = rows.numel()
-    for name, t in (("k", k), ("v", v)):
-        if t.get_device() != dev or t.dtype != k.dtype or t.dtype not in _DTYPES or t.shape != (n, heads, d):
-            raise ValueError(f"{name} must be [rows, num_kv_heads, head_dim] in bf16 or fp32 on the pool's device, k and v alike")
-        if n > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != d) or (n > 1 and t.stride(0) < heads * d)):
-            raise ValueError(f"{name}: the heads of a row must follow each other without gaps, and rows not overlap")
+def _row_stride(name: str, t: torch.Tensor, n: int, heads: int, d: int, dtype: torch.dtype, dev: int) -> int:
+    """Elements between the rows of ``[n, heads, d]``; raises unless the heads of a row are packed."""
+    if t.dtype != dtype or dtype not in _DTYPES or t.get_device() != dev or t.shape != (n, heads, d):
+        raise ValueError(f"{name} must be [rows, num_kv_heads, head_dim] in bf16 or fp32 on the pool's device, k and v alike")
+    s0, s1, s2 = t.stride()
+    if n > 1 and s2 == 1 and s1 == d and s0 >= heads * d:
+        return s0
+    if n > 0 and (s2 != 1 or (heads > 1 and s1 != d) or (n > 1 and s0 < heads * d)):
+        raise ValueError(f"{name}: the heads of a row must follow each other without gaps, and rows not overlap")
+    return s0 if n > 1 else heads * d
+
+
+def _row_args(pool, d, k, v, rows, k_scale, v_scale, status) -> TsQuantRowsArgs:
+    # A decode step's rows cost the device less than a generous host path costs Python: one look at each property.
+    dev, (pool_rows, heads, _) = pool.get_device(), pool.shape
+    n, dtype = rows.numel(), k.dtype
+    ks, vs = _row_stride("k", k, n, heads, d, dtype, dev), _row_stride("v", v, n, heads, d, dtype, dev)
     _check_ints(dev, (("rows", rows), ("status", status)))
-    ks, vs = (k.stride(0), v.stride(0)) if n > 1 else (heads * d, heads * d)
-    return TsQuantRowsArgs(_ROWS_ARGS_SIZE, dev, _DTYPES[k.dtype], heads, d, n, k.data_ptr(), v.data_ptr(), ks, vs,
+    return TsQuantRowsArgs(_ROWS_ARGS_SIZE, dev, _DTYPES[dtype], heads, d, n, k.data_ptr(), v.data_ptr(), ks, vs,
                            rows.data_ptr(), pool.data_ptr(), pool_rows, k_scale, v_scale,
                            None if status is None else status.data_ptr(), _raw_stream(dev))
 
@@ -75,8 +88,8 @@ def kv4_write(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: torch.
     """Quantise ``k, v [n, num_kv_heads, head_dim]`` (bf16 or fp32, rows may be strided) into the pool rows
     ``rows [n]`` (``out_cache_loc`` of the serving stack).  A row outside the pool is skipped and reported; a row that
     is listed twice is left with a mixture of the two."""
-    a = _row_args(pool, k, v, rows, k_scale, v_scale, status)
-    check(_lib.load().ts_quant_write(C.byref(a)), "ts_quant_write")
+    a = _row_args(pool, _check_pool(pool), k, v, rows, k_scale, v_scale, status)
+    check(_lib_().ts_quant_write(C.byref(a)), "ts_quant_write")
 
 
 def kv4_read(pool: torch.Tensor, rows: torch.Tensor, dtype: torch.dtype = torch.bfloat16, k_scale: float = 1.0,
@@ -87,12 +100,14 @@ def kv4_read(pool: torch.Tensor, rows: torch.Tensor, dtype: torch.dtype = torch.
     zeros and is reported."""
     d = _check_pool(pool)
     shape = (rows.numel(), pool.shape[1], d)
-    if k is None:
-        k = torch.empty(shape, dtype=dtype, device=pool.device)
-    if v is None:
-        v = torch.empty(shape, dtype=dtype, device=pool.device)
-    a = _row_args(pool, k, v, rows, k_scale, v_scale, status)
-    check(_lib.load().ts_quant_read(C.byref(a)), "ts_quant_read")
+    if k is None and v is None:
+        k, v = pool.new_empty((2, *shape), dtype=dtype).unbind(0)
+    elif k is None:
+        k = pool.new_empty(shape, dtype=dtype)
+    elif v is None:
+        v = pool.new_empty(shape, dtype=dtype)
+    a = _row_args(pool, d, k, v, rows, k_scale, v_scale, status)
+    check(_lib_().ts_quant_read(C.byref(a)), "ts_quant_read")
     return k, v
 
 
@@ -101,7 +116,7 @@ def kv4_attend_workspace(batch: int, num_q_heads: int, head_dim: int, device: in
     key = (device, batch, num_q_heads, head_dim)
     if key not in _workspace_bytes:
         n = C.c_size_t()
-        check(_lib.load().ts_quant_attend_workspace(device, batch, num_q_heads, head_dim, C.byref(n)), "ts_quant_attend_workspace")
+        check(_lib_().ts_quant_attend_workspace(device, batch, num_q_heads, head_dim, C.byref(n)), "ts_quant_attend_workspace")
         _workspace_bytes[key] = n.value
     return _workspace_bytes[key]
 
@@ -120,29 +135,31 @@ def kv4_attend(q: torch.Tensor, pool: torch.Tensor, req_to_token: torch.Tensor, 
     ``workspace``: uint8, at least :func:`kv4_attend_workspace` bytes, for callers that must not allocate; calls that
     may run at the same time need one each.  By default every call takes its own from PyTorch's allocator."""
     d, dev, (pool_rows, hkv, _) = _check_pool(pool), pool.get_device(), pool.shape
-    batch = q.shape[0]
-    hq = q.numel() // (batch * d) if batch > 0 else hkv
+    i32, dtype, batch, total = torch.int32, q.dtype, q.shape[0], q.numel()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if not (q.get_device() == out.get_device() == dev and q.dtype == out.dtype and q.dtype in _DTYPES
-            and q.is_contiguous() and out.is_contiguous() and q.numel() == out.numel() == batch * hq * d and hq % hkv == 0):
+    hq = total // (batch * d) if batch > 0 else hkv
+    if not (q.get_device() == out.get_device() == dev and dtype == out.dtype and dtype in _DTYPES
+            and q.is_contiguous() and out.is_contiguous() and total == out.numel() == batch * hq * d and hq % hkv == 0):
         raise ValueError("q/out must be contiguous [batch, num_q_heads*head_dim] in bf16 or fp32 on the pool's device")
-    if req_to_token.dim() != 2 or req_to_token.stride(1) != 1 or req_to_token.dtype != torch.int32 or req_to_token.get_device() != dev:
+    table = req_to_token.stride()
+    if len(table) != 2 or table[1] != 1 or req_to_token.dtype != i32 or req_to_token.get_device() != dev:
         raise ValueError("req_to_token must be int32 [max_reqs, max_ctx] with unit inner stride on the pool's device")
     if req_pool_indices.numel() != batch or seq_lens.numel() != batch:
         raise ValueError("req_pool_indices and seq_lens must have one entry per request")
     _check_ints(dev, (("req_pool_indices", req_pool_indices), ("seq_lens", seq_lens), ("status", status)))
     if batch == 0:
         return out
-    nbytes = kv4_attend_workspace(batch, hq, d, dev)
+    nbytes = _workspace_bytes.get((dev, batch, hq, d)) or kv4_attend_workspace(batch, hq, d, dev)
     if workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=pool.device)
+        workspace = pool.new_empty(nbytes)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous on the pool's device")
-    a = TsQuantAttendArgs(_ATTEND_ARGS_SIZE, dev, _DTYPES[q.dtype], batch, hq, hkv, d, req_to_token.shape[0], q.data_ptr(),
-                          pool.data_ptr(), pool_rows, req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[1],
-                          req_pool_indices.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), sm_scale, logit_cap, rope_base,
-                          rope_scale, k_scale, v_scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+    max_reqs, max_ctx = req_to_token.shape
+    a = TsQuantAttendArgs(_ATTEND_ARGS_SIZE, dev, _DTYPES[dtype], batch, hq, hkv, d, max_reqs, q.data_ptr(), pool.data_ptr(),
+                          pool_rows, req_to_token.data_ptr(), table[0], max_ctx, req_pool_indices.data_ptr(),
+                          seq_lens.data_ptr(), out.data_ptr(), sm_scale, logit_cap, rope_base, rope_scale, k_scale, v_scale,
+                          workspace.data_ptr(), workspace.numel() * workspace.element_size(),
                           None if status is None else status.data_ptr(), _raw_stream(dev))
-    check(_lib.load().ts_quant_attend(C.byref(a)), "ts_quant_attend")
+    check(_lib_().ts_quant_attend(C.byref(a)), "ts_quant_attend")
     return out
