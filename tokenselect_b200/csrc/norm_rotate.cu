@@ -3,11 +3,11 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w,   (y_i, y_{i+D/2}) -> (y_i cos - y_{i+D/2} sin, y_{i+D/2} cos + y_i sin)
 //
 // What bounds it: HBM (a row is read once, written once, a key row twice) and, for a few tokens, the launch.  Eight lanes
-// hold the rows of up to four neighbouring heads of a token: lane l the elements [P l, P l + P) of both halves of each
+// hold the rows of two (D = 64: four) neighbouring heads of a token: lane l the elements [P l, P l + P) of both halves of each
 // (P = D/16), that is both members of its rotation pairs, so the rotation exchanges nothing and the norm three shuffles, and
 // the angles (an integer product each, rope.cuh, and in bf16 the fast sine and cosine, whose 2^-20 is far below the output's
-// 2^-9) are evaluated once for four heads.  All rows are requested before the first is used.  No table, no shared memory, no
-// barrier: the groups of eight lanes are independent.
+// 2^-9) are evaluated once for them.  All rows are requested before the first is used.  In fp32 it runs at 95 % of the copy
+// rate; in bf16, with half the bytes for the same arithmetic, the instructions come close, and pairs of numbers halve them.
 #include "ptx.cuh"
 #include "rope.cuh"
 
@@ -16,7 +16,9 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormLanes = 8;                                  // lanes a row
-constexpr int kNormHeads = 4;                                  // rows of a group of lanes
+// Rows of a group of lanes: 32 elements a thread (8192 tokens, 32 + 8 heads of 128 in bf16: 40.2 us with four rows a thread,
+// 36.4 with two, 62 with one; heads of 64: 18.6 with four, 19.9 with two).
+template <int D> constexpr int kNormHeads = 256 / D;
 
 struct NormParams {
     const void* q;
@@ -75,7 +77,10 @@ __device__ __forceinline__ void store_row(T* dst, const float (&x)[P]) {
 
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_constant__ NormParams p) {
-    constexpr int P = D / 2 / kNormLanes;
+    constexpr int P = D / 2 / kNormLanes, R = kNormHeads<D>;
+    __shared__ unsigned long long freqs[D / 2];                // (lanes read different ones: the parameters' bank would serve them one by one)
+    if (threadIdx.x < D / 2) freqs[threadIdx.x] = p.freqs.f[threadIdx.x];
+    __syncthreads();
     const int lane = threadIdx.x % kNormLanes;
     const unsigned long long group = (unsigned long long)blockIdx.x * (kNormThreads / kNormLanes) + threadIdx.x / kNormLanes;
     const bool mine = group < p.groups;                        // the others keep their warp's shuffles company
@@ -83,13 +88,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_
     const long long t = (long long)t64;
     const unsigned part = mine ? (unsigned)(group - t64 * p.per_token) : 0u;
     const bool is_q = part < p.groups_q;
-    const int h0 = (int)(is_q ? part : part - p.groups_q) * kNormHeads, count = min(kNormHeads, (is_q ? p.hq : p.hkv) - h0);
+    const int h0 = (int)(is_q ? part : part - p.groups_q) * R, count = min(R, (is_q ? p.hq : p.hkv) - h0);
     const T* src = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_stride : reinterpret_cast<const T*>(p.k) + t * p.k_stride) + h0 * D + P * lane;
     const T* w = reinterpret_cast<const T*>(is_q ? p.q_weight : p.k_weight);
     wait_for_predecessor();
-    float lo[kNormHeads][P], hi[kNormHeads][P];
+    float lo[R][P], hi[R][P];
 #pragma unroll
-    for (int i = 0; i < kNormHeads; ++i) {                     // behind the last head: that one again
+    for (int i = 0; i < R; ++i) {                     // behind the last head: that one again
         load_row<T, P, WIDE>(src + min(i, count - 1) * D, lo[i]);
         load_row<T, P, WIDE>(src + min(i, count - 1) * D + D / 2, hi[i]);
     }
@@ -100,16 +105,26 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_
             load_row<T, P, WIDE>(w + D / 2 + P * lane, b);
         }
 #pragma unroll
-        for (int i = 0; i < kNormHeads; ++i) {
-            float sum = 0.f;
+        for (int i = 0; i < R; ++i) {
+            uint64_t squares = 0ull;
 #pragma unroll
-            for (int e = 0; e < P; ++e) sum += lo[i][e] * lo[i][e] + hi[i][e] * hi[i][e];
+            for (int e = 0; e < P; e += 2) {
+                const uint64_t x = pack_f32x2(lo[i][e], lo[i][e + 1]), y = pack_f32x2(hi[i][e], hi[i][e + 1]);
+                squares = fma_f32x2(y, y, fma_f32x2(x, x, squares));
+            }
+            float sum, odd;
+            unpack_f32x2(squares, sum, odd);
+            sum += odd;
 #pragma unroll
             for (int off = 1; off < kNormLanes; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             if (w != nullptr) {
                 const float r = rsqrtf(sum * (1.f / D) + p.eps);
+                const uint64_t r2 = pack_f32x2(r, r);
 #pragma unroll
-                for (int e = 0; e < P; ++e) { lo[i][e] = lo[i][e] * r * a[e]; hi[i][e] = hi[i][e] * r * b[e]; }
+                for (int e = 0; e < P; e += 2) {
+                    unpack_f32x2(mul_f32x2(mul_f32x2(pack_f32x2(lo[i][e], lo[i][e + 1]), r2), pack_f32x2(a[e], a[e + 1])), lo[i][e], lo[i][e + 1]);
+                    unpack_f32x2(mul_f32x2(mul_f32x2(pack_f32x2(hi[i][e], hi[i][e + 1]), r2), pack_f32x2(b[e], b[e + 1])), hi[i][e], hi[i][e + 1]);
+                }
             }
         }
     }
@@ -118,7 +133,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_
     if (!is_q && p.k_plain != nullptr) {
         T* plain = reinterpret_cast<T*>(p.k_plain) + at;
 #pragma unroll
-        for (int i = 0; i < kNormHeads; ++i)
+        for (int i = 0; i < R; ++i)
             if (i < count) {
                 store_row<T, P, WIDE>(plain + i * D, lo[i]);
                 store_row<T, P, WIDE>(plain + i * D + D / 2, hi[i]);
@@ -127,19 +142,21 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotate_kernel(const __grid_
     if (p.positions != nullptr) {
         const long long pos = p.positions[t];
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-            const float2 cs = sizeof(T) == 2 ? cos_sin_fast(pos, p.freqs.f[P * lane + e]) : cos_sin(pos, p.freqs.f[P * lane + e]);
+        for (int e = 0; e < P; e += 2) {
+            const unsigned long long f0 = freqs[P * lane + e], f1 = freqs[P * lane + e + 1];
+            const float2 cs0 = sizeof(T) == 2 ? cos_sin_fast(pos, f0) : cos_sin(pos, f0), cs1 = sizeof(T) == 2 ? cos_sin_fast(pos, f1) : cos_sin(pos, f1);
+            const uint64_t c = pack_f32x2(cs0.x, cs1.x), s = pack_f32x2(cs0.y, cs1.y), minus_s = pack_f32x2(-cs0.y, -cs1.y);
 #pragma unroll
-            for (int i = 0; i < kNormHeads; ++i) {
-                const float x = lo[i][e], y = hi[i][e];
-                lo[i][e] = x * cs.x - y * cs.y;
-                hi[i][e] = y * cs.x + x * cs.y;
+            for (int i = 0; i < R; ++i) {
+                const uint64_t x = pack_f32x2(lo[i][e], lo[i][e + 1]), y = pack_f32x2(hi[i][e], hi[i][e + 1]);
+                unpack_f32x2(fma_f32x2(y, minus_s, mul_f32x2(x, c)), lo[i][e], lo[i][e + 1]);
+                unpack_f32x2(fma_f32x2(x, s, mul_f32x2(y, c)), hi[i][e], hi[i][e + 1]);
             }
         }
     }
     T* out = reinterpret_cast<T*>(is_q ? p.q_out : p.k_out) + at;
 #pragma unroll
-    for (int i = 0; i < kNormHeads; ++i)
+    for (int i = 0; i < R; ++i)
         if (i < count) {
             store_row<T, P, WIDE>(out + i * D, lo[i]);
             store_row<T, P, WIDE>(out + i * D + D / 2, hi[i]);
@@ -178,8 +195,9 @@ extern "C" int ts_norm_rotate(const ts_norm_rotate_args* a) {
     p.positions = a->positions; p.q_weight = a->q_weight; p.k_weight = a->k_weight;
     p.q_out = a->q_out; p.k_out = a->k_out; p.k_plain = a->k_plain;
     p.hq = a->hq; p.hkv = a->hkv; p.eps = a->eps;
-    p.groups_q = (a->hq + kNormHeads - 1) / kNormHeads;
-    p.per_token = p.groups_q + (a->hkv + kNormHeads - 1) / kNormHeads;
+    const int heads = a->head_dim == 128 ? kNormHeads<128> : kNormHeads<64>;
+    p.groups_q = (a->hq + heads - 1) / heads;
+    p.per_token = p.groups_q + (a->hkv + heads - 1) / heads;
     p.groups = (unsigned long long)a->tokens * p.per_token;
     if (p.groups > ((1ull << 31) - 1) * (kNormThreads / kNormLanes)) return TS_ERR_CAPACITY;      // blocks of one launch
     if (a->positions) p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);

@@ -302,28 +302,6 @@ __device__ __noinline__ void prompt_row(const PromptParams& p, int first, int ro
     for (int e = 0; e < E; ++e) out[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
 }
 
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack_f32x2(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // 2^x of two numbers on the multipliers, for x >= -125 (below, 2^-125): 2^n 2^f with n the nearest whole number and 2^f a
 // polynomial of degree 3 (Remez exchange: 7.5e-5 relative on [-1/2, 1/2], a twentieth of the weight's rounding to bf16).
 __device__ __forceinline__ uint64_t exp2_f32x2(uint64_t x) {
