@@ -30,6 +30,7 @@ struct QuantAttendParams {
     float* part_o;                                             // [slots][hq][d] unnormalised
     float2* part_ml;                                           // [slots][hq] (maximum in base-2 units, sum)
     int batch, hq, hkv, group, max_reqs, pieces;
+    int step_units;                                            // units that a CTA takes in one step
     float sm_scale, logit_cap, v_scale;                        // sm_scale includes the pool's scale of K
     int* status;
     TurnFreqs freqs;
@@ -65,8 +66,9 @@ __device__ __forceinline__ void count_units(const QuantAttendParams& p, int* sta
     }
     __syncthreads();
 }
-// Pieces in use: no piece is empty, so every slot between a request's first and last one is written.
-__device__ __forceinline__ int used_pieces(int units, int pieces) { return min(units, pieces); }
+// Pieces in use: no piece is empty, so every slot between a request's first and last one is written.  And none is shorter than
+// what a CTA's warps take in their first step anyway: fewer partial results then cost nothing.
+__device__ __forceinline__ int used_pieces(const QuantAttendParams& p, int units) { return min((units + p.step_units - 1) / p.step_units, p.pieces); }
 __device__ __forceinline__ int piece_start(int units, int piece, int pieces) { return (int)((long long)units * piece / pieces); }
 // The piece that owns unit u: the last one that starts at or before it.
 __device__ __forceinline__ int piece_of(int u, int units, int pieces) { return (int)(((long long)(u + 1) * pieces - 1) / units); }
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
     wait_for_predecessor();
     count_units(p, start);
     const int units = start[p.batch];
-    const int pieces = used_pieces(units, p.pieces);
+    const int pieces = used_pieces(p, units);
     if ((int)blockIdx.x >= pieces) return;
     const int u_end = piece_start(units, blockIdx.x + 1, pieces);
     int u = piece_start(units, blockIdx.x, pieces);
@@ -275,6 +277,14 @@ __host__ __device__ __forceinline__ int row_pitch(int heads) {
 }
 
 template <int D>
+__host__ __device__ __forceinline__ int ring_space(int heads) { return kQtBytes - (int)sizeof(QuantTcSmem<D>) - heads * D * 16; }
+// Warps that share a head's units.
+template <int D>
+__host__ __device__ __forceinline__ int shares_of(int heads) {
+    const int most = ring_space<D>(heads) / (kQtMinStages * kUnit * row_pitch<D>(heads));
+    return kQtWarps / heads < most ? kQtWarps / heads : most;
+}
+template <int D>
 constexpr bool rings_fit() {
     for (int heads = 1; heads <= kQtWarps; ++heads) {
         const int bytes = heads * QuantRow<D>::kBytes, pitch = bytes + ((16 - bytes) & 127);
@@ -336,7 +346,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     {
         const int pair = threadIdx.x % HALF, owner = pair / (D / 8), r = pair % (D / 8);
         const unsigned long long f = p.freqs.f[pair];
-        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit && warp < kQtWarps; i += 32 * kQtWarps / HALF) {
+        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit; i += kQtThreads / HALF) {
             const float2 cs = cos_sin_fast(i, f);
             __half* row = reinterpret_cast<__half*>(sm.turn[i]);
             const int swap = (i & 1) * (D == 128 ? 4 : 2);
@@ -349,11 +359,10 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     const int hpc = (p.hkv + gridDim.y - 1) / gridDim.y;       // KV heads of a CTA
     const int head0 = blockIdx.y * hpc, heads = min(hpc, p.hkv - head0);
     const int pitch = row_pitch<D>(hpc), stage_bytes = kUnit * pitch;
-    const int ring_space = kQtBytes - (int)sizeof(QuantTcSmem<D>) - hpc * D * 16;
-    const int share = min(kQtWarps / hpc, ring_space / (kQtMinStages * stage_bytes));           // warps of a head
+    const int share = shares_of<D>(hpc);
     uint4* queries = reinterpret_cast<uint4*>(dyn + sizeof(QuantTcSmem<D>));                   // [hpc][D/32][32]: pairs of a lane, bf16
     unsigned char* rings = reinterpret_cast<unsigned char*>(queries + hpc * D);
-    const int stages = min(kQtMaxStages, ring_space / (share * stage_bytes));
+    const int stages = min(kQtMaxStages, ring_space<D>(hpc) / (share * stage_bytes));
     const bool requests = warp >= kQtWarps;
     const int my_head = warp % hpc, kv = head0 + my_head, my_share = warp / hpc;
     const bool busy = !requests && my_share < share && my_head < heads;
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     wait_for_predecessor();
     count_units(p, sm.start);                                  // ends with a barrier: the table and the barriers are complete too
-    const int units = sm.start[p.batch], pieces = used_pieces(units, p.pieces);
+    const int units = sm.start[p.batch], pieces = used_pieces(p, units);
     if ((int)blockIdx.x >= pieces) return;
     const int u_end = piece_start(units, blockIdx.x + 1, pieces);
     const unsigned char* head_pool = p.pool + (long long)head0 * Row::kBytes;
@@ -709,19 +718,19 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
 }
 
 // ------------------------------------------------------------------------------------------------
-// Join the partial results: grid (hq, batch), one warp per partial in flight
+// Join the partial results: grid (hq, batch); a warp has eight of them in flight, so that 128 are one round trip
 // ------------------------------------------------------------------------------------------------
-constexpr int kQmThreads = 256;
+constexpr int kQmThreads = 512;
 template <typename T, int D>
 __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_constant__ QuantAttendParams p) {
-    constexpr int VEC = D / 32, NW = kQmThreads / 32, kAhead = 4;
+    constexpr int VEC = D / 32, NW = kQmThreads / 32, kAhead = 8;
     __shared__ int start[kQaMaxBatch + 1];
     __shared__ float s_acc[NW][D];
     __shared__ float2 s_ml[NW];
     const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     wait_for_predecessor();
     count_units(p, start);
-    const int units = start[p.batch], pieces = used_pieces(units, p.pieces);
+    const int units = start[p.batch], pieces = used_pieces(p, units);
     float m = -INFINITY, l = 0.f, acc[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
@@ -804,8 +813,9 @@ cudaError_t launch_attend_plain(const QuantAttendParams& p, cudaStream_t stream)
     return launch_chained(quant_merge_kernel<float, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
 }
 template <int D, bool CAP, int PIECE>
-cudaError_t launch_attend_tc(const QuantAttendParams& p, cudaStream_t stream) {
+cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
     static SmemConfig configured = {};
+    p.step_units = 2 * shares_of<D>((p.hkv + tc_head_blocks(p.hkv) - 1) / tc_head_blocks(p.hkv));
     cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP, PIECE>, kQtBytes, configured);
     if (e != cudaSuccess) return e;
     e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), kQtBytes, stream, p);
@@ -862,7 +872,7 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)(pieces + a->batch) * a->hq * a->head_dim);
     p.batch = a->batch; p.hq = a->hq; p.hkv = a->hkv; p.group = a->hq / a->hkv; p.max_reqs = a->max_reqs; p.pieces = pieces;
     p.sm_scale = a->sm_scale * a->k_scale; p.logit_cap = a->logit_cap; p.v_scale = a->v_scale;
-    p.status = a->status;
+    p.status = a->status; p.step_units = 1;
     p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;
