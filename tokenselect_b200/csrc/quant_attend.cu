@@ -30,7 +30,7 @@ struct QuantAttendParams {
     float* part_o;                                             // [slots][hq][d] unnormalised
     float2* part_ml;                                           // [slots][hq] (maximum in base-2 units, sum)
     int batch, hq, hkv, group, max_reqs, pieces;
-    int step_units;                                            // units that a CTA takes in one step
+    int step_units, share;                                     // units that a CTA takes in one step; partial results of a slot
     float sm_scale, logit_cap, v_scale;                        // sm_scale includes the pool's scale of K
     int* status;
     TurnFreqs freqs;
@@ -261,10 +261,10 @@ constexpr int kQtMacro = 8;                                    // units of a mac
 constexpr int kQtMinStages = 4, kQtMaxStages = 8, kQtBytes = 232448;          // (dynamic shared memory)
 
 template <int D>
-struct QuantTcSmem {                                           // behind it: the heads' queries, then the rings
+struct QuantTcSmem {                                           // behind it: the rings
     uint4 turn[kQtMacro * kUnit][D / 8];                       // per key of a macro tile: cosines, sines of the pairs, fp16
     float2 base[kQtWarps][D / 2];                              // per warp: (cos, sin) of the query's distance to the tile
-    float2 ml[kQtWarps][8];
+    uint4 q[kQtWarps][D / 32][32];                             // per warp and lane: its pairs of its head's query, bf16
     uint64_t full[kQtWarps][kQtMaxStages], empty[kQtWarps][kQtMaxStages];
     int start[kQaMaxBatch + 1];
     int pad[3];
@@ -277,19 +277,18 @@ __host__ __device__ __forceinline__ int row_pitch(int heads) {
 }
 
 template <int D>
-__host__ __device__ __forceinline__ int ring_space(int heads) { return kQtBytes - (int)sizeof(QuantTcSmem<D>) - heads * D * 16; }
+__host__ __device__ __forceinline__ int ring_space() { return kQtBytes - (int)sizeof(QuantTcSmem<D>); }
 // Warps that share a head's units.
 template <int D>
 __host__ __device__ __forceinline__ int shares_of(int heads) {
-    const int most = ring_space<D>(heads) / (kQtMinStages * kUnit * row_pitch<D>(heads));
+    const int most = ring_space<D>() / (kQtMinStages * kUnit * row_pitch<D>(heads));
     return kQtWarps / heads < most ? kQtWarps / heads : most;
 }
 template <int D>
 constexpr bool rings_fit() {
     for (int heads = 1; heads <= kQtWarps; ++heads) {
         const int bytes = heads * QuantRow<D>::kBytes, pitch = bytes + ((16 - bytes) & 127);
-        if (kQtBytes - (int)sizeof(QuantTcSmem<D>) - heads * D * 16 < kQtMinStages * kUnit * pitch) return false;
-        if (kQtBytes - (int)sizeof(QuantTcSmem<D>) - heads * D * 16 < kQtWarps * 8 * D * 4) return false;       // the warps' results at the end
+        if (kQtBytes - (int)sizeof(QuantTcSmem<D>) < kQtMinStages * kUnit * pitch) return false;
     }
     return true;
 }
@@ -359,10 +358,9 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     const int hpc = (p.hkv + gridDim.y - 1) / gridDim.y;       // KV heads of a CTA
     const int head0 = blockIdx.y * hpc, heads = min(hpc, p.hkv - head0);
     const int pitch = row_pitch<D>(hpc), stage_bytes = kUnit * pitch;
-    const int share = shares_of<D>(hpc);
-    uint4* queries = reinterpret_cast<uint4*>(dyn + sizeof(QuantTcSmem<D>));                   // [hpc][D/32][32]: pairs of a lane, bf16
-    unsigned char* rings = reinterpret_cast<unsigned char*>(queries + hpc * D);
-    const int stages = min(kQtMaxStages, ring_space<D>(hpc) / (share * stage_bytes));
+    const int share = p.share;                                 // warps of a head
+    unsigned char* rings = dyn + sizeof(QuantTcSmem<D>);
+    const int stages = min(kQtMaxStages, ring_space<D>() / (share * stage_bytes));
     const bool requests = warp >= kQtWarps;
     const int my_head = warp % hpc, kv = head0 + my_head, my_share = warp / hpc;
     const bool busy = !requests && my_share < share && my_head < heads;
@@ -499,9 +497,8 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 }
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
-                    // (the warps of a head write the same values to the same place)
-                    queries[(my_head * 2 * NW + w) * 32 + lane] = make_uint4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]);
-                    queries[(my_head * 2 * NW + NW + w) * 32 + lane] = make_uint4(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3]);
+                    sm.q[warp][w][lane] = make_uint4(x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]);
+                    sm.q[warp][NW + w][lane] = make_uint4(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3]);
                 }
             }
             // a column of S^T is a query head: this thread's columns are heads 2t and 2t + 1
@@ -526,7 +523,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                     __syncwarp();
 #pragma unroll
                     for (int w = 0; w < NW; ++w) {
-                        const uint4 x4 = queries[(my_head * 2 * NW + w) * 32 + lane], y4 = queries[(my_head * 2 * NW + NW + w) * 32 + lane];
+                        const uint4 x4 = sm.q[warp][w][lane], y4 = sm.q[warp][NW + w][lane];
                         const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -676,38 +673,23 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 l1 += __shfl_xor_sync(0xffffffffu, l1, off);
             }
         }
-        // join the warps of a head; the rings are free
-        __syncthreads();
+        // This warp's partial result.  Elements of a head in the order in which the lanes hold them (element_at), so that eight
+        // lanes' pairs are 64 bytes side by side.
         if (busy) {
-            float* mine = reinterpret_cast<float*>(rings) + warp * 8 * D;
+            const long long slot = (long long)(blockIdx.x + b) * share + my_share;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                *reinterpret_cast<float2*>(mine + (2 * t) * D + g * (D / 8) + 2 * i) = make_float2(o[i][0], o[i][2]);
-                *reinterpret_cast<float2*>(mine + (2 * t + 1) * D + g * (D / 8) + 2 * i) = make_float2(o[i][1], o[i][3]);
-            }
-        }
-        if (busy && g == 0) { sm.ml[warp][2 * t] = make_float2(m0, l0); sm.ml[warp][2 * t + 1] = make_float2(m1, l1); }
-        __syncthreads();
-        if (busy) {
-            const long long slot = blockIdx.x + b;
-            for (int i = my_share * 32 + lane; i < p.group * D; i += share * 32) {
-                const int h = i / D, d = i - h * D;
-                float mm = -1e30f;
-                for (int w = 0; w < share; ++w) mm = fmaxf(mm, sm.ml[w * hpc + my_head][h].x);
-                float sum = 0.f, l = 0.f;
-                for (int w = 0; w < share; ++w) {
-                    const float2 ml = sm.ml[w * hpc + my_head][h];
-                    const float weight = exp2_fast(ml.x - mm);
-                    sum += reinterpret_cast<const float*>(rings)[(w * hpc + my_head) * 8 * D + h * D + d] * weight;
-                    l += ml.y * weight;
+            for (int k = 0; k < 2; ++k) {
+                const int head = 2 * t + k;
+                if (head < p.group) {
+                    const long long at = slot * p.hq + kv * p.group + head;
+                    if (steps > 0) {
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(p.part_o + at * D + 16 * i + 2 * g) = make_float2(o[i][k], o[i][2 + k]);
+                    }
+                    if (g == 0) p.part_ml[at] = k == 0 ? make_float2(m0, l0) : make_float2(m1, l1);
                 }
-                const long long at = slot * p.hq + kv * p.group + h;
-                p.part_o[at * D + d] = sum;
-                if (d == 0) p.part_ml[at] = make_float2(mm, l);
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next rows come behind the reads above
-        __syncthreads();
         u0 = u1;
     }
     if (requests && __any_sync(0xffffffffu, dead) && lane < share)       // given up: the copies still have to land (or time out)
@@ -721,7 +703,8 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
 // Join the partial results: grid (hq, batch); a warp has eight of them in flight, so that 128 are one round trip
 // ------------------------------------------------------------------------------------------------
 constexpr int kQmThreads = 512;
-template <typename T, int D>
+// LANES: elements in the order of the tensor-core kernel's lanes.
+template <typename T, int D, bool LANES>
 __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_constant__ QuantAttendParams p) {
     constexpr int VEC = D / 32, NW = kQmThreads / 32, kAhead = 8;
     __shared__ int start[kQaMaxBatch + 1];
@@ -735,8 +718,9 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
 #pragma unroll
     for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
     if (start[b] < start[b + 1]) {
-        const int c_end = piece_of(start[b + 1] - 1, units, pieces);
-        for (int c0 = piece_of(start[b], units, pieces) + warp; c0 <= c_end; c0 += NW * kAhead) {
+        const int c_first = piece_of(start[b], units, pieces), count = (piece_of(start[b + 1] - 1, units, pieces) - c_first + 1) * p.share;
+        const long long first = (long long)(c_first + b) * p.share;
+        for (int c0 = warp; c0 < count; c0 += NW * kAhead) {
             float x[kAhead][VEC];
             float2 ml[kAhead];
 #pragma unroll
@@ -745,8 +729,8 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
                 ml[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) x[i][v] = 0.f;
-                if (c <= c_end) {
-                    const long long at = (long long)(c + b) * p.hq + h;
+                if (c < count) {
+                    const long long at = (first + c) * p.hq + h;
                     ml[i] = __ldcg(p.part_ml + at);
                     const float* src = p.part_o + at * D + VEC * lane;
                     if constexpr (VEC == 4) {
@@ -771,7 +755,7 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
                 const float w = exp2f(ml[i].x - base);
                 l += ml[i].y * w;
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) acc[v] += x[i][v] * w;
+                for (int v = 0; v < VEC; ++v) acc[v] += w > 0.f || w != w ? x[i][v] * w : 0.f;     // (a warp without units leaves no elements)
             }
             m = mn;
         }
@@ -791,8 +775,9 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
             r += s_acc[w][e] * wgt;
             ll += s_ml[w].y * wgt;
         }
+        const int d = LANES ? (e & 15) / 2 * (D / 8) + e / 16 * 2 + (e & 1) : e;
         // an empty request: no row, sum 0, zeros
-        reinterpret_cast<T*>(p.out)[((long long)b * p.hq + h) * D + e] = from_f32<T>(start[b] < start[b + 1] ? r / ll * p.v_scale : 0.f);
+        reinterpret_cast<T*>(p.out)[((long long)b * p.hq + h) * D + d] = from_f32<T>(start[b] < start[b + 1] ? r / ll * p.v_scale : 0.f);
     }
 }
 
@@ -803,24 +788,31 @@ int attend_pieces(int dtype, int hkv, int sms) {
     return dtype == TS_DTYPE_BF16 ? (sms + tc_head_blocks(hkv) - 1) / tc_head_blocks(hkv) : 4 * sms;
 }
 
-size_t partial_bytes(int pieces, int batch, int hq, int d) { return (size_t)(pieces + batch) * hq * (d + 2) * sizeof(float); }
+// At most (a KV head serves up to eight query heads, a CTA's warps are shared out over its KV heads).
+size_t partial_slots(int sms, int batch, int hq) {
+    const int hkv = (hq + 7) / 8, share = hkv < kQtWarps ? kQtWarps / hkv : 1;
+    const size_t tc = (size_t)(sms + batch) * share, plain = 4 * sms + batch;
+    return tc > plain ? tc : plain;
+}
+size_t partial_bytes(int sms, int batch, int hq, int d) { return partial_slots(sms, batch, hq) * hq * (d + 2) * sizeof(float); }
 
 template <int D>
 cudaError_t launch_attend_plain(const QuantAttendParams& p, cudaStream_t stream) {
     const int nsub = (p.group + kQpHeads - 1) / kQpHeads, per_cta = kQpThreads / 32;
     const cudaError_t e = launch_chained(quant_attend_plain_kernel<float, D>, dim3(p.pieces, (p.hkv * nsub + per_cta - 1) / per_cta), dim3(kQpThreads), 0, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_chained(quant_merge_kernel<float, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+    return launch_chained(quant_merge_kernel<float, D, false>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
 }
 template <int D, bool CAP, int PIECE>
 cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
     static SmemConfig configured = {};
-    p.step_units = 2 * shares_of<D>((p.hkv + tc_head_blocks(p.hkv) - 1) / tc_head_blocks(p.hkv));
+    p.share = shares_of<D>((p.hkv + tc_head_blocks(p.hkv) - 1) / tc_head_blocks(p.hkv));
+    p.step_units = 2 * p.share;
     cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP, PIECE>, kQtBytes, configured);
     if (e != cudaSuccess) return e;
     e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), kQtBytes, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_chained(quant_merge_kernel<__nv_bfloat16, D>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+    return launch_chained(quant_merge_kernel<__nv_bfloat16, D, true>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
 }
 template <int D, bool CAP>
 cudaError_t launch_attend_bf16(const QuantAttendParams& p, cudaStream_t stream) {
@@ -840,7 +832,7 @@ extern "C" int ts_quant_attend_workspace(int32_t device, int32_t batch, int32_t 
     if (head_dim != 64 && head_dim != 128) return TS_ERR_UNSUPPORTED;
     const int sms = sms_of(device);
     if (sms <= 0) return TS_ERR_CUDA;
-    *bytes = partial_bytes(4 * sms, batch, hq, head_dim);      // the most that any type and head count takes
+    *bytes = partial_bytes(sms, batch, hq, head_dim);          // whatever the type and the number of KV heads
     return TS_OK;
 }
 
@@ -861,7 +853,7 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     const int sms = sms_of(a->device);
     if (sms <= 0) return TS_ERR_CUDA;
     const int pieces = attend_pieces(a->dtype, a->hkv, sms);
-    if (a->workspace_bytes < partial_bytes(pieces, a->batch, a->hq, a->head_dim)) return TS_ERR_CAPACITY;
+    if (a->workspace_bytes < partial_bytes(sms, a->batch, a->hq, a->head_dim)) return TS_ERR_CAPACITY;
     const DeviceScope scope(a->device);
     if (!scope.ok) return TS_ERR_CUDA;
     QuantAttendParams p;
@@ -869,10 +861,10 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     p.rtt = a->req_to_token; p.rtt_stride = a->req_to_token_stride; p.max_ctx = a->max_ctx;
     p.req_pool_indices = a->req_pool_indices; p.seq_lens = a->seq_lens; p.out = a->out;
     p.part_o = static_cast<float*>(a->workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)(pieces + a->batch) * a->hq * a->head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + partial_slots(sms, a->batch, a->hq) * a->hq * a->head_dim);
     p.batch = a->batch; p.hq = a->hq; p.hkv = a->hkv; p.group = a->hq / a->hkv; p.max_reqs = a->max_reqs; p.pieces = pieces;
     p.sm_scale = a->sm_scale * a->k_scale; p.logit_cap = a->logit_cap; p.v_scale = a->v_scale;
-    p.status = a->status; p.step_units = 1;
+    p.status = a->status; p.step_units = 1; p.share = 1;
     p.freqs = turn_freqs(a->rope_base, a->rope_scale, a->head_dim);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(a->stream);
     cudaError_t e;
