@@ -32,33 +32,43 @@ struct QuantRowsParams {
 };
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load_block(const T* src, float (&x)[kQuantBlock]) {
+__device__ __forceinline__ void load_block(const T* src, T (&x)[kQuantBlock]) {
     if constexpr (WIDE) {
-        constexpr int kPer = 16 / (int)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < kQuantBlock / kPer; ++i) {
-            alignas(16) T raw[kPer];
-            *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + i * kPer);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) x[i * kPer + e] = to_f32<T>(raw[e]);
-        }
+        for (int i = 0; i < (int)sizeof(x) / 16; ++i) reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(src)[i];
     } else {
 #pragma unroll
-        for (int e = 0; e < kQuantBlock; ++e) x[e] = to_f32<T>(src[e]);
+        for (int e = 0; e < kQuantBlock; ++e) x[e] = src[e];
+    }
+}
+
+// Bits of the largest magnitude; an infinity or a NaN counts as the largest.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(const T (&x)[kQuantBlock]) {
+    if constexpr (sizeof(T) == 2) {                            // two at a time
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+        uint32_t top = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int e = 1; e < kQuantBlock / 2; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+        return max(top & 0xffffu, top >> 16) << 16;
+    } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < kQuantBlock; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        return top;
     }
 }
 
 // The block's codes in `w`; returns its scale.
-__device__ __forceinline__ uint32_t quantise_block(const float (&x)[kQuantBlock], float g, uint2& w) {
-    uint32_t top = 0;                                          // largest magnitude; as bits, so that NaN counts as the largest
-#pragma unroll
-    for (int e = 0; e < kQuantBlock; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+template <typename T>
+__device__ __forceinline__ uint32_t quantise_block(const T (&x)[kQuantBlock], float g, uint2& w) {
+    const uint32_t top = largest<T>(x);
     w = make_uint2(0u, 0u);
     if (top >= 0x7f800000u) return 0x7fu;                      // an infinity or a NaN: the scale is NaN
-    const float inv_g = 1.f / g, most = __uint_as_float(top) * inv_g;
+    const float most = __uint_as_float(top) * (1.f / g);
     const uint32_t scale = f32_to_e4m3(fminf(__fdiv_rn(most, 6.f), 448.f));
     if (scale == 0) return 0;
-    const float s = e4m3_to_f32(scale);
+    const float s = e4m3_to_f32(scale) * g;
     float y[2][8];
     if (most < 1e30f) {
         // Sixteen quotients by one divisor: Markstein's correction (1990) of the product with the rounded reciprocal gives the
@@ -66,12 +76,12 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&x)[kQuantBlock]
         const float inv_s = __fdiv_rn(1.f, s);
 #pragma unroll
         for (int e = 0; e < kQuantBlock; ++e) {
-            const float v = x[e] * inv_g, q = v * inv_s;
+            const float v = to_f32<T>(x[e]), q = v * inv_s;
             y[e >> 3][e & 7] = fmaf(fmaf(-q, s, v), inv_s, q);
         }
-    } else {                                                   // far beyond what the scale can hold, where v may be infinite
+    } else {                                                   // far beyond what the scale can hold: the quotient may be infinite
 #pragma unroll
-        for (int e = 0; e < kQuantBlock; ++e) y[e >> 3][e & 7] = __fdiv_rn(x[e] * inv_g, s);
+        for (int e = 0; e < kQuantBlock; ++e) y[e >> 3][e & 7] = __fdiv_rn(to_f32<T>(x[e]), s);
     }
     w = make_uint2(f32x8_to_e2m1(y[0]), f32x8_to_e2m1(y[1]));
     return scale;
@@ -100,51 +110,59 @@ __global__ void __launch_bounds__(kRowsThreads) quant_write_kernel(const QuantRo
     const int row = p.rows[at.i];
     if (row < 0 || row >= p.pool_rows) { report(p.status, TS_ERR_BAD_SLOT); return; }
     const T* src = at.is_v ? reinterpret_cast<const T*>(p.v) + at.i * p.v_stride : reinterpret_cast<const T*>(p.k) + at.i * p.k_stride;
-    float x[kQuantBlock];
+    alignas(16) T x[kQuantBlock];
     load_block<T, WIDE>(src + at.head * D + at.part * kQuantBlock, x);
     uint2 w;
-    const uint32_t scale = quantise_block(x, at.is_v ? p.v_scale : p.k_scale, w);
+    const uint32_t scale = quantise_block<T>(x, at.is_v ? p.v_scale : p.k_scale, w);
     unsigned char* dst = p.pool + ((long long)row * p.hkv + at.head) * Row::kBytes;
     *reinterpret_cast<uint2*>(dst + (at.is_v ? Row::kV : 0) + at.part * 8) = w;
     dst[(at.is_v ? Row::kVScales : Row::kKScales) + at.part] = (unsigned char)scale;
 }
 
+// Two threads share two neighbouring blocks, half of each for either: what the two store at a time lies side by side (with a
+// block a thread, a store fills 16 of every 32 bytes).
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads) quant_read_kernel(const QuantRowsParams p) {
     using Row = QuantRow<D>;
     const unsigned b = blockIdx.x * kRowsThreads + threadIdx.x;
     wait_for_predecessor();
     if (b >= p.blocks) return;
-    const BlockPlace at = block_place<D>(b, p.hkv);
+    BlockPlace at = block_place<D>(b, p.hkv);
+    const int half = at.part & 1;
+    at.part &= ~1;
     const int row = p.rows[at.i];
-    uint2 w = make_uint2(0u, 0u);
-    uint32_t scale = 0;
+    uint32_t w[2] = {0u, 0u}, scale[2] = {0u, 0u};
     if (row >= 0 && row < p.pool_rows) {
         const unsigned char* src = p.pool + ((long long)row * p.hkv + at.head) * Row::kBytes;
-        w = *reinterpret_cast<const uint2*>(src + (at.is_v ? Row::kV : 0) + at.part * 8);
-        scale = src[(at.is_v ? Row::kVScales : Row::kKScales) + at.part];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            w[i] = *reinterpret_cast<const uint32_t*>(src + (at.is_v ? Row::kV : 0) + (at.part + i) * 8 + half * 4);
+            scale[i] = src[(at.is_v ? Row::kVScales : Row::kKScales) + at.part + i];
+        }
     } else {
         report(p.status, TS_ERR_BAD_SLOT);
     }
-    const float s = e4m3_to_f32(scale) * (at.is_v ? p.v_scale : p.k_scale);
     T* dst = (at.is_v ? reinterpret_cast<T*>(p.v) + at.i * p.v_stride : reinterpret_cast<T*>(p.k) + at.i * p.k_stride) +
-             at.head * D + at.part * kQuantBlock;
-    uint32_t h[2][4];
-    e2m1x8_to_f16(w.x, h[0]);
-    e2m1x8_to_f16(w.y, h[1]);
-    alignas(16) T out[kQuantBlock];
+             at.head * D + at.part * kQuantBlock + half * 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float2 f = half2_to_float2(h[e >> 2][e & 3]);
-        out[2 * e] = from_f32<T>(f.x * s);
-        out[2 * e + 1] = from_f32<T>(f.y * s);
-    }
-    if constexpr (WIDE) {
+    for (int i = 0; i < 2; ++i) {
+        const float s = e4m3_to_f32(scale[i]) * (at.is_v ? p.v_scale : p.k_scale);
+        uint32_t h[4];
+        e2m1x8_to_f16(w[i], h);
+        alignas(16) T out[8];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(out) / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(out)[i];
-    } else {
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = half2_to_float2(h[e]);
+            out[2 * e] = from_f32<T>(f.x * s);
+            out[2 * e + 1] = from_f32<T>(f.y * s);
+        }
+        if constexpr (WIDE) {
 #pragma unroll
-        for (int e = 0; e < kQuantBlock; ++e) dst[e] = out[e];
+            for (int j = 0; j < (int)sizeof(out) / 16; ++j) reinterpret_cast<uint4*>(dst + i * kQuantBlock)[j] = reinterpret_cast<const uint4*>(out)[j];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[i * kQuantBlock + e] = out[e];
+        }
     }
 }
 
@@ -153,7 +171,7 @@ cudaError_t launch_rows_t(const QuantRowsParams& p, bool write, cudaStream_t str
     const uintptr_t bits = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | (uintptr_t)(p.k_stride * sizeof(T)) |
                            (uintptr_t)(p.v_stride * sizeof(T));
     const bool wide = bits % 16 == 0;
-    const dim3 grid((unsigned)((p.blocks + kRowsThreads - 1) / kRowsThreads)), block(kRowsThreads);
+    const dim3 grid((p.blocks + kRowsThreads - 1) / kRowsThreads), block(kRowsThreads);
     if (write) return wide ? launch_chained(quant_write_kernel<T, D, true>, grid, block, 0, stream, p)
                            : launch_chained(quant_write_kernel<T, D, false>, grid, block, 0, stream, p);
     return wide ? launch_chained(quant_read_kernel<T, D, true>, grid, block, 0, stream, p)

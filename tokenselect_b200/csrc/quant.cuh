@@ -16,7 +16,8 @@ struct QuantRow {
     static constexpr int kBytes = 2 * (kCodes + kScales);      // 9 D / 8
 };
 
-// Eight 4-bit floats (the lower half of each byte first) as pairs of fp16, exact.
+// Eight 4-bit floats (the lower half of each byte first) as pairs of fp16, exact.  `w` has to be loaded as a whole word: with a
+// byte or a 16-bit load zero-extended into it, nvcc 12.9 made code that gave zeros.
 __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
