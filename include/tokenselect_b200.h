@@ -479,7 +479,7 @@ typedef struct ts_prompt_args {
     const void* v;
     int64_t q_stride, k_stride, v_stride;
     const int32_t* cu_seqlens;     /* [batch+1] */
-    void* out;                     /* [tokens, hq, head_dim] */
+    void* out;                     /* [tokens, hq, head_dim]; overlaps none of the inputs */
     int32_t* status;
     void* stream;
 } ts_prompt_args;

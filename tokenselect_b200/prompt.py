@@ -112,6 +112,8 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_out("out", out, q)
+        if n > 0 and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+            raise ValueError("out must not be one of the inputs")
     a = TsPromptArgs(_PROMPT_ARGS_SIZE, dev, _DTYPES[dtype], n, cu_seqlens.numel() - 1, hq, hkv, d, sm_scale, logit_cap,
                      q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, cu_seqlens.data_ptr(), out.data_ptr(),
                      None if status is None else status.data_ptr(), _raw_stream(dev))
