@@ -11,6 +11,8 @@ namespace {
 
 constexpr int kPromptMaxBatch = 4096;
 
+template <bool B> struct Flag { static constexpr bool value = B; };
+
 struct PromptParams {
     const void* q;
     const void* k;
@@ -32,17 +34,21 @@ __device__ __forceinline__ int2 sequence_of(const PromptParams& p, int b) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// CUDA cores
+// CUDA cores: fp32
 // ------------------------------------------------------------------------------------------------
-// A CTA takes 64 query tokens of one head, key tiles of 64 pass through shared memory in fp32.  Thread (ty, tx) holds
-// rows 4 ty .. 4 ty + 3 and, of S, columns tx + 16 j; of O, elements 4 tx + 64 j.
-constexpr int kPpThreads = 256, kPpTile = 64;
+// A CTA takes 32 query tokens of one head; keys and values pass through shared memory in tiles of 64, K of the next tile
+// arriving under the second product and V under the first.  Thread (ty, tx) holds rows 4 ty .. 4 ty + 3 and, of S, columns
+// tx + 16 j; of O, elements 4 tx + 64 j.  What bounds it: the multipliers (and, for few tokens, the CTA with the most keys,
+// hence the small tile); products take two numbers an instruction, so that the loads of their operands find a place
+// between them.
+constexpr int kPpThreads = 128, kPpRows = 32, kPpTile = 64;
 
 template <int D>
 struct PromptPlainSmem {
-    float q[kPpTile][D + 4];
-    float kv[kPpTile][D + 4];                                  // the tile's keys, then its values
-    float p[kPpTile][kPpTile + 4];
+    float q[kPpRows][D + 4];
+    float k[kPpTile][D + 4];
+    float v[kPpTile][D + 4];
+    float p[kPpTile][kPpRows + 4];                             // [key][row]
     int tiles[kPpThreads];
     int found[3];                                              // first token, length, tile
 };
@@ -53,7 +59,7 @@ template <int D>
 __device__ __forceinline__ bool find_tile(const PromptParams& p, int tile, PromptPlainSmem<D>& sm) {
     const int per = (p.batch + kPpThreads - 1) / kPpThreads, b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += (sequence_of(p, b).y + kPpTile - 1) / kPpTile;
+    for (int b = b0; b < b1; ++b) sum += (sequence_of(p, b).y + kPpRows - 1) / kPpRows;
     sm.tiles[threadIdx.x] = sum;
     if (threadIdx.x == 0) sm.found[1] = 0;
     __syncthreads();
@@ -62,7 +68,7 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int tile, Promp
     if (tile >= before && tile < before + sum) {
         for (int b = b0; b < b1; ++b) {
             const int2 s = sequence_of(p, b);
-            const int n = (s.y + kPpTile - 1) / kPpTile;
+            const int n = (s.y + kPpRows - 1) / kPpRows;
             if (tile < before + n) {
                 sm.found[0] = s.x; sm.found[1] = s.y; sm.found[2] = n - 1 - (tile - before);
                 break;
@@ -74,20 +80,25 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int tile, Promp
     return sm.found[1] > 0;
 }
 
-// Rows [row0, row0 + 64) of a [tokens, heads, D] tensor into shared memory; zeros from row `end` on.
-template <typename T, int D>
-__device__ __forceinline__ void stage_rows(float (*dst)[D + 4], const T* src, long long stride, int row0, int end) {
-    constexpr int kPer = 16 / (int)sizeof(T), kVecs = D / kPer;
-    for (int i = threadIdx.x; i < kPpTile * kVecs; i += kPpThreads) {
-        const int r = i / kVecs, c = i % kVecs * kPer;
-        alignas(16) T raw[kPer];
-        *reinterpret_cast<uint4*>(raw) = row0 + r < end ? *reinterpret_cast<const uint4*>(src + (row0 + r) * stride + c) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) dst[r][c + e] = to_f32<T>(raw[e]);
+// Rows [row0, row0 + ROWS) of a [tokens, heads, D] tensor into shared memory; zeros from row `end` on.
+template <int D, int ROWS>
+__device__ __forceinline__ void request_rows(float (*dst)[D + 4], const float* src, long long stride, int row0, int end) {
+    constexpr int kVecs = D / 4;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < ROWS * kVecs; i += kPpThreads) {
+        const int r = i / kVecs, c = i % kVecs * 4;
+        const bool in = row0 + r < end;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&dst[r][c])), "l"(src + (in ? (row0 + r) * stride + c : 0)), "r"(in ? 16 : 0) : "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void rows_here() {                  // all but the last N requests
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncthreads();
 }
 
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kPpThreads) prompt_plain_kernel(const PromptParams p) {
     extern __shared__ __align__(16) unsigned char dyn[];
     PromptPlainSmem<D>& sm = *reinterpret_cast<PromptPlainSmem<D>*>(dyn);
@@ -95,91 +106,107 @@ __global__ void __launch_bounds__(kPpThreads) prompt_plain_kernel(const PromptPa
     const int h = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     wait_for_predecessor();
     if (!find_tile<D>(p, blockIdx.x, sm)) return;
-    const int first = sm.found[0], len = sm.found[1], row0 = sm.found[2] * kPpTile;      // in the sequence
-    const T* q = reinterpret_cast<const T*>(p.q) + (long long)first * p.q_stride + (long long)h * D;
-    const T* k = reinterpret_cast<const T*>(p.k) + (long long)first * p.k_stride + (long long)(h / p.group) * D;
-    const T* v = reinterpret_cast<const T*>(p.v) + (long long)first * p.v_stride + (long long)(h / p.group) * D;
-    stage_rows<T, D>(sm.q, q, p.q_stride, row0, len);
-    float m[4], l[4], o[4][OJ][4];
+    const int first = sm.found[0], len = sm.found[1], row0 = sm.found[2] * kPpRows;      // in the sequence
+    const float* q = reinterpret_cast<const float*>(p.q) + (long long)first * p.q_stride + (long long)h * D;
+    const float* k = reinterpret_cast<const float*>(p.k) + (long long)first * p.k_stride + (long long)(h / p.group) * D;
+    const float* v = reinterpret_cast<const float*>(p.v) + (long long)first * p.v_stride + (long long)(h / p.group) * D;
+    request_rows<D, kPpRows>(sm.q, q, p.q_stride, row0, len);
+    request_rows<D, kPpTile>(sm.k, k, p.k_stride, 0, len);
+    request_rows<D, kPpTile>(sm.v, v, p.v_stride, 0, len);
+    const int end = min(row0 + kPpRows, len);                  // keys that the tile sees
+    float m[4], l[4];
+    uint64_t o[4][OJ][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < OJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
+        for (int j = 0; j < OJ; ++j) o[i][j][0] = o[i][j][1] = 0ull;
     }
-    for (int key0 = 0; key0 <= row0; key0 += kPpTile) {
-        __syncthreads();
-        stage_rows<T, D>(sm.kv, k, p.k_stride, key0, len);
-        __syncthreads();
-        float s[4][4];
+    for (int key0 = 0; key0 < end; key0 += kPpTile) {
+        rows_here<1>();                                        // Q and K
+        uint64_t s2[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+            for (int j = 0; j < 4; ++j) s2[i][j] = 0ull;
 #pragma unroll 4
         for (int d = 0; d < D; d += 4) {
-            float4 a[4], b[4];
+            ulonglong2 a[4], b[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(&sm.q[4 * ty + i][d]);
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(&sm.q[4 * ty + i][d]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(&sm.kv[tx + 16 * j][d]);
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(&sm.k[tx + 16 * j][d]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] += a[i].x * b[j].x + a[i].y * b[j].y + a[i].z * b[j].z + a[i].w * b[j].w;
+                for (int j = 0; j < 4; ++j) s2[i][j] = fma_f32x2(a[i].y, b[j].y, fma_f32x2(a[i].x, b[j].x, s2[i][j]));
         }
-        const bool diagonal = key0 == row0;
+        __syncthreads();                                       // K has been read
+        request_rows<D, kPpTile>(sm.k, k, p.k_stride, key0 + kPpTile, end);
+        const bool diagonal = key0 + kPpTile > row0;
+        float pe[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float mx = -INFINITY;
+            const int lim = row0 + 4 * ty + i - key0;          // the row sees keys up to this one of the tile
+            float s[4], mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float x = s[i][j] * p.sm_scale;
+                float even, odd;
+                unpack_f32x2(s2[i][j], even, odd);
+                float x = (even + odd) * p.sm_scale;
                 if (p.logit_cap > 0.f) x = p.logit_cap * tanhf(x / p.logit_cap);
-                s[i][j] = diagonal && tx + 16 * j > 4 * ty + i ? -INFINITY : x * 1.4426950408889634f;
-                mx = fmaxf(mx, s[i][j]);
+                s[j] = diagonal && tx + 16 * j > lim ? -INFINITY : x * 1.4426950408889634f;
+                mx = fmaxf(mx, s[j]);
             }
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m[i] - base);
             m[i] = mn;
-            float sum = 0.f;
+            l[i] *= corr;                                      // this thread's columns; joined at the end
+            const uint64_t corr2 = pack_f32x2(corr, corr);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float pe = exp2f(s[i][j] - base);
-                sum += pe;
-                sm.p[4 * ty + i][tx + 16 * j] = pe;
+                pe[j][i] = exp2f(s[j] - base);
+                l[i] += pe[j][i];
             }
-            l[i] = l[i] * corr + sum;                          // this thread's columns; joined at the end
 #pragma unroll
-            for (int j = 0; j < OJ; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][j][e] *= corr;
+            for (int j = 0; j < OJ; ++j) {
+                o[i][j][0] = mul_f32x2(o[i][j][0], corr2);
+                o[i][j][1] = mul_f32x2(o[i][j][1], corr2);
+            }
         }
-        __syncthreads();
-        stage_rows<T, D>(sm.kv, v, p.v_stride, key0, len);
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(&sm.p[tx + 16 * j][4 * ty]) = make_float4(pe[j][0], pe[j][1], pe[j][2], pe[j][3]);
+        rows_here<1>();                                        // V; and P
         // On the diagonal a masked weight is 0, but 0 times a later token's infinity is not: those products are left out.
-        const int keys = diagonal ? min(kPpTile, len - key0) : kPpTile;
-        for (int c = 0; c < keys; ++c) {
-            float4 b[OJ];
+        const int keys = min(kPpTile, end - key0);
+        auto products = [&](auto masked) {
+#pragma unroll 4
+            for (int c = 0; c < keys; ++c) {
+                ulonglong2 b[OJ];
 #pragma unroll
-            for (int j = 0; j < OJ; ++j) b[j] = *reinterpret_cast<const float4*>(&sm.kv[c][4 * tx + 64 * j]);
+                for (int j = 0; j < OJ; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(&sm.v[c][4 * tx + 64 * j]);
+                const float4 a4 = *reinterpret_cast<const float4*>(&sm.p[c][4 * ty]);
+                const float a[4] = {a4.x, a4.y, a4.z, a4.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = sm.p[4 * ty + i][c];
-                if (!diagonal || c <= 4 * ty + i) {
+                for (int i = 0; i < 4; ++i) {
+                    if (!decltype(masked)::value || key0 + c <= row0 + 4 * ty + i) {
+                        const uint64_t a2 = pack_f32x2(a[i], a[i]);
 #pragma unroll
-                    for (int j = 0; j < OJ; ++j) {
-                        o[i][j][0] += a * b[j].x; o[i][j][1] += a * b[j].y; o[i][j][2] += a * b[j].z; o[i][j][3] += a * b[j].w;
+                        for (int j = 0; j < OJ; ++j) {
+                            o[i][j][0] = fma_f32x2(a2, b[j].x, o[i][j][0]);
+                            o[i][j][1] = fma_f32x2(a2, b[j].y, o[i][j][1]);
+                        }
                     }
                 }
             }
-        }
+        };
+        if (diagonal) products(Flag<true>()); else products(Flag<false>());
+        __syncthreads();                                       // V and P have been read
+        request_rows<D, kPpTile>(sm.v, v, p.v_stride, key0 + kPpTile, end);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");       // (zeros, requested behind the last tile)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float sum = l[i];
@@ -187,12 +214,24 @@ __global__ void __launch_bounds__(kPpThreads) prompt_plain_kernel(const PromptPa
         for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const int row = row0 + 4 * ty + i;
         if (row >= len) continue;
-        T* out = reinterpret_cast<T*>(p.out) + ((long long)(first + row) * p.hq + h) * D;
+        float* out = reinterpret_cast<float*>(p.out) + ((long long)(first + row) * p.hq + h) * D;
 #pragma unroll
-        for (int j = 0; j < OJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) out[4 * tx + 64 * j + e] = from_f32<T>(o[i][j][e] / sum);
+        for (int j = 0; j < OJ; ++j) {
+            float x[4];
+            unpack_f32x2(o[i][j][0], x[0], x[1]);
+            unpack_f32x2(o[i][j][1], x[2], x[3]);
+            *reinterpret_cast<float4*>(out + 4 * tx + 64 * j) = make_float4(x[0] / sum, x[1] / sum, x[2] / sum, x[3] / sum);
+        }
     }
+}
+
+template <int D>
+cudaError_t launch_prompt_plain(const PromptParams& p, cudaStream_t stream) {
+    static SmemConfig configured = {};
+    constexpr size_t kSmem = sizeof(PromptPlainSmem<D>);
+    const cudaError_t e = ensure_dynamic_smem(prompt_plain_kernel<D>, kSmem, configured);
+    if (e != cudaSuccess) return e;
+    return launch_chained(prompt_plain_kernel<D>, dim3(p.tokens / kPpRows + p.batch, p.hq), dim3(kPpThreads), kSmem, stream, p);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -319,7 +358,6 @@ __device__ __forceinline__ uint64_t exp2_f32x2(uint64_t x) {
     unpack_f32x2(n, na, nb);
     return pack_f32x2(__int_as_float(__float_as_int(ya) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(yb) + (__float_as_int(nb) << 23)));
 }
-template <bool B> struct Flag { static constexpr bool value = B; };
 
 // True for one lane of a converged warp.  (With `lane == 0` in its place the compiler does not know the code behind it to be
 // uniform and moves every operand of every product into uniform registers anew.)
@@ -686,15 +724,6 @@ cudaError_t launch_prompt_tc(const PromptParams& p, int sms, cudaStream_t stream
     return launch_chained(prompt_tc_kernel<D, CAP>, dim3((unsigned)(items < sms ? items : sms)), dim3(kPtThreads), kSmem, stream, p, q, k, v);
 }
 
-template <typename T, int D>
-cudaError_t launch_prompt_plain(const PromptParams& p, cudaStream_t stream) {
-    static SmemConfig configured = {};
-    constexpr size_t kSmem = sizeof(PromptPlainSmem<D>);
-    const cudaError_t e = ensure_dynamic_smem(prompt_plain_kernel<T, D>, kSmem, configured);
-    if (e != cudaSuccess) return e;
-    return launch_chained(prompt_plain_kernel<T, D>, dim3(p.tokens / kPpTile + p.batch, p.hq), dim3(kPpThreads), kSmem, stream, p);
-}
-
 }  // namespace
 }  // namespace ts
 
@@ -724,7 +753,7 @@ extern "C" int ts_prompt_attend(const ts_prompt_args* a) {
     const int sms = sms_of(a->device);
     if (sms <= 0) return TS_ERR_CUDA;
     const bool cap = a->logit_cap > 0.f;
-    if (a->dtype == TS_DTYPE_F32) e = a->head_dim == 128 ? launch_prompt_plain<float, 128>(p, s) : launch_prompt_plain<float, 64>(p, s);
+    if (a->dtype == TS_DTYPE_F32) e = a->head_dim == 128 ? launch_prompt_plain<128>(p, s) : launch_prompt_plain<64>(p, s);
     else if (a->head_dim == 128) e = cap ? launch_prompt_tc<128, true>(p, sms, s) : launch_prompt_tc<128, false>(p, sms, s);
     else e = cap ? launch_prompt_tc<64, true>(p, sms, s) : launch_prompt_tc<64, false>(p, sms, s);
     return e == cudaSuccess ? TS_OK : TS_ERR_CUDA;
