@@ -59,9 +59,9 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tens
     n, hq, d = shape
     qs, ks = _token_stride("q", q, n, d, dtype, dev), _token_stride("k", k, n, d, dtype, dev)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != dtype or w.get_device() != dev or w.shape != (d,) or not w.is_contiguous()):
+        if w is not None and (w.dtype != dtype or w.get_device() != dev or w.numel() != d or not w.is_contiguous()):
             raise ValueError(f"{name} must be [head_dim] of q's type on q's device")
-    if positions is not None and (positions.dtype != torch.int32 or positions.get_device() != dev or positions.shape != (n,)
+    if positions is not None and (positions.dtype != torch.int32 or positions.get_device() != dev or positions.numel() != n
                                   or not positions.is_contiguous()):
         raise ValueError("positions must be a contiguous int32 tensor [tokens] on q's device")
     packed = torch.contiguous_format

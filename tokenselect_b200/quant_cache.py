@@ -55,8 +55,9 @@ def _check_pool(pool: torch.Tensor) -> int:
 
 
 def _check_ints(device: int, named) -> None:
+    i32 = torch.int32
     for name, t in named:
-        if t is not None and (t.dtype != torch.int32 or t.get_device() != device or not t.is_contiguous()):
+        if t is not None and (t.dtype != i32 or t.get_device() != device or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous int32 tensor on the pool's device")
 
 
@@ -100,12 +101,10 @@ def kv4_read(pool: torch.Tensor, rows: torch.Tensor, dtype: torch.dtype = torch.
     zeros and is reported."""
     d = _check_pool(pool)
     shape = (rows.numel(), pool.shape[1], d)
-    if k is None and v is None:
-        k, v = pool.new_empty((2, *shape), dtype=dtype).unbind(0)
-    elif k is None:
-        k = pool.new_empty(shape, dtype=dtype)
-    elif v is None:
-        v = pool.new_empty(shape, dtype=dtype)
+    if k is None:
+        k = pool.new_empty(shape, dtype=dtype if v is None else v.dtype)
+    if v is None:
+        v = torch.empty_like(k, memory_format=torch.contiguous_format)
     a = _row_args(pool, d, k, v, rows, k_scale, v_scale, status)
     check(_lib_().ts_quant_read(C.byref(a)), "ts_quant_read")
     return k, v
