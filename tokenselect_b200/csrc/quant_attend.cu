@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 // Eight computing warps with their operands in registers do as well as sixteen with some of them spilled.
 constexpr int kQtWarps = 8, kQtLoaders = 4, kQtThreads = 32 * (kQtWarps + kQtLoaders);
 constexpr int kQtBulkBytes = 400;                              // bulk copies for rows of at least this many
+constexpr int kQtComputeRegs = 224, kQtLoadRegs = 56;          // of a launch with 168 a thread: 2 * 224 + 56 = 3 * 168
 constexpr int kQtMacro = 8;                                    // units of a macro tile
 // Stages of a ring: a step holds two while the two behind it arrive, so fewer than four would wait for themselves.
 constexpr int kQtMinStages = 4, kQtMaxStages = 8, kQtBytes = 232448;          // (dynamic shared memory)
@@ -331,6 +332,27 @@ __device__ __forceinline__ void load_words(const unsigned char* src, uint32_t (&
     else w[0] = *reinterpret_cast<const uint32_t*>(src);
 }
 
+// What a CTA takes of one request: units [u0, u1), dealt out to the warps of a head in macro tiles of `per` units.
+struct Segment {
+    int b, n, first, u1, per;                                  // request, its length and first unit
+    const int* table;
+    __device__ __forceinline__ int units_of(int u0, int w, int share) const {      // of share w
+        const int round = share * per, whole = (u1 - u0) / round, rest = u1 - u0 - whole * round;
+        return whole * per + min(per, max(0, rest - w * per));
+    }
+};
+__device__ __forceinline__ Segment segment_at(const QuantAttendParams& p, const int* start, int u0, int u_end, int share) {
+    Segment s;
+    s.b = request_of(start, p.batch, u0);
+    s.n = p.seq_lens[s.b];
+    s.first = start[s.b];
+    s.u1 = min(u_end, start[s.b + 1]);
+    s.table = p.rtt + (long long)p.req_pool_indices[s.b] * p.rtt_stride;
+    const int units = s.u1 - u0, rounds = (units + share * kQtMacro - 1) / (share * kQtMacro);
+    s.per = (units + share * rounds - 1) / (share * rounds);
+    return s;
+}
+
 // PIECE: 0, rows by bulk copies; 16 or 8, by pieces of that many bytes.
 template <int D, bool CAP, int PIECE>
 __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __grid_constant__ QuantAttendParams p) {
@@ -341,14 +363,15 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
     // The turns of a macro tile's keys.  16-byte unit 4 c + t (c: cosines' then sines' words) holds what thread t reads; the units
-    // of odd keys are exchanged by halves so that a read of two keys by eight lanes meets eight different bank groups.
+    // of every other pair of keys are exchanged by fours so that a read of two keys by eight lanes meets eight different bank
+    // groups (key_of).
     {
         const int pair = threadIdx.x % HALF, owner = pair / (D / 8), r = pair % (D / 8);
         const unsigned long long f = p.freqs.f[pair];
         for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit; i += kQtThreads / HALF) {
             const float2 cs = cos_sin_fast(i, f);
             __half* row = reinterpret_cast<__half*>(sm.turn[i]);
-            const int swap = (i & 1) * (D == 128 ? 4 : 2);
+            const int swap = (i & 2) * 2;
             // D = 128: a thread's 16 pairs are two units of cosines and two of sines; D = 64: its 8 pairs one of each
             const int uc = ((r >> 3) * 4 + owner) ^ swap, us = ((NW + (r >> 3)) * 4 + owner) ^ swap;
             row[uc * 8 + (r & 7)] = __float2half_rn(cs.x);
@@ -380,31 +403,20 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     const int width = heads * Row::kBytes;                     // bytes of a row that this CTA takes
     unsigned char* ring = rings + min(my_share, share - 1) * stages * stage_bytes;
     const uint32_t full = smem_u32(sm.full[min(my_share, share - 1)]), empty = smem_u32(sm.empty[min(my_share, share - 1)]);
-    int stage = 0;                                             // next stage to read
-    uint32_t phase = 0;                                        // parity of its barrier
-    int before = 0;                                            // a requesting warp's lane w: units of share w in the requests so far
     bool dead = false;
     const unsigned long long f0 = p.freqs.f[lane], f1 = D == 128 ? p.freqs.f[(lane + 32) % HALF] : 0ull;
 
     int u0 = piece_start(units, blockIdx.x, pieces);
-    while (u0 < u_end) {
-        const int b = request_of(sm.start, p.batch, u0);
-        const int n = p.seq_lens[b], first = sm.start[b], u1 = min(u_end, sm.start[b + 1]);
-        const int* table = p.rtt + (long long)p.req_pool_indices[b] * p.rtt_stride;
-        // macro tiles of `per` units go round the warps of a head
-        const int rounds = (u1 - u0 + share * kQtMacro - 1) / (share * kQtMacro), per = (u1 - u0 + share * rounds - 1) / (share * rounds);
-        auto units_of = [&](int w) {                           // of share w
-            const int round = share * per, whole = (u1 - u0) / round, rest = u1 - u0 - whole * round;
-            return whole * per + min(per, max(0, rest - w * per));
-        };
-        const int steps = busy ? units_of(my_share) : 0, skip = (share - 1) * per;
-        float o[MT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-
-        if (requests) {
+    if (requests) {
+        // ---------------- requests ----------------
+        // (these warps leave their registers to the computing ones)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtLoadRegs));
+        int before = 0;                                        // lane w: units of share w in the segments so far
+        while (u0 < u_end) {
+            const Segment seg = segment_at(p, sm.start, u0, u_end, share);
+            const int b = seg.b, n = seg.n, first = seg.first, u1 = seg.u1, per = seg.per;
+            const int* table = seg.table;
+            auto units_of = [&](int w) { return seg.units_of(u0, w, share); };
             // Lane w keeps the place of share w: unit `at` of its units, counted over all requests, goes into stage at % stages and is
             // requested by warp at % 4 of these.  Lanes 16 (w & 1) + r of ahead[w / 2] hold the number of row r of this warp's next
             // unit (or none), read when the one before was requested.
@@ -430,6 +442,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 const bool ready = at < end && (dead || test_phase(smem_u32(&sm.empty[lane % kQtWarps][stage_in]), (at / stages & 1) ^ 1));
                 unsigned todo = __ballot_sync(0xffffffffu, ready);
                 if (todo == 0) {
+                    __nanosleep(100);                          // (leaves the issue slots to the computing warps)
                     if (clock64() - idle_since > kWaitCycles) { report(p.status, TS_ERR_DEVICE_TIMEOUT); dead = true; }
                     dead = __any_sync(0xffffffffu, dead);
                     continue;
@@ -470,7 +483,29 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 idle_since = clock64();
             }
             before = end;
+            u0 = u1;
         }
+        if (__any_sync(0xffffffffu, dead) && lane < share)     // given up: the copies still have to land (or time out)
+            for (int i = max(before - stages, 0); i < before; ++i) {
+                bool gone = false;
+                wait_phase(smem_u32(&sm.full[lane][i % stages]), i / stages & 1, p.status, gone);
+            }
+        return;
+    }
+    // ---------------- products ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQtComputeRegs));
+    int stage = 0;                                             // next stage to read
+    uint32_t phase = 0;                                        // parity of its barrier
+    while (u0 < u_end) {
+        const Segment seg = segment_at(p, sm.start, u0, u_end, share);
+        const int b = seg.b, n = seg.n, first = seg.first, u1 = seg.u1, per = seg.per;
+        const int* table = seg.table;
+        const int steps = busy ? seg.units_of(u0, my_share, share) : 0, skip = (share - 1) * per;
+        float o[MT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         if (steps > 0) {
             // the query of head g, of which a quad's thread turns its own pairs; scaled by a power of two to below 2
             const bool real = g < p.group;
@@ -506,6 +541,8 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
             const float mul0 = __shfl_sync(0xffffffffu, unit_scale, 8 * t) * per_log, mul1 = __shfl_sync(0xffffffffu, unit_scale, 8 * t + 4) * per_log;
 
             uint32_t qa[4 * NW], qb[4 * NW];
+            const int swap = (key_of(g) & 2) * 2;
+            const uint32_t blk_k = t * (D / 8) / kQuantBlock, pick = blk_k | (blk_k + 4) << 4;      // bytes of the row's K scales
             int in_macro = 0, unit = u0 + my_share * per;      // units of the macro tile done; the next one
 
             for (int s = 0; s < steps;) {
@@ -549,14 +586,27 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const unsigned char* row = st[j] + key_of(g + 8 * r) * pitch + Row::kKScales + t * (D / 8) / kQuantBlock;
-                        const uint32_t two = e4m3x2_to_f16(row[0] | (uint32_t)row[D / 32] << 8);
+                        // all scales of the key's row at once; of them the thread's two
+                        const unsigned char* row = st[j] + key_of(g + 8 * r) * pitch + Row::kKScales;
+                        uint32_t lo, hi;
+                        if constexpr (D == 128) { const uint2 x = *reinterpret_cast<const uint2*>(row); lo = x.x; hi = x.y; }
+                        else { lo = *reinterpret_cast<const uint32_t*>(row); hi = lo >> 16; }
+                        const uint32_t two = e4m3x2_to_f16(__byte_perm(lo, hi, pick));
                         s_lo[j][r] = __byte_perm(two, two, 0x1010);
                         s_hi[j][r] = __byte_perm(two, two, 0x3232);
                         sc[j][2 * r] = 0.f;
                         sc[j][2 * r + 1] = 0.f;
                     }
                 const int in_second = min(in_macro + 1, kQtMacro - 1);
+                uint32_t k_lo[2][2][NW], k_hi[2][2][NW];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const unsigned char* row = st[j] + key_of(g + 8 * r) * pitch + t * 4 * NW;
+                        load_words<D>(row, k_lo[j][r]);
+                        load_words<D>(row + D / 4, k_hi[j][r]);
+                    }
 #pragma unroll
                 for (int w = 0; w < NW; ++w)
 #pragma unroll
@@ -564,14 +614,12 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                         uint32_t a_lo[2][4], a_hi[2][4];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const int key = key_of(g + 8 * r), swap = r * (D == 128 ? 4 : 2);      // r is the key's parity
-                            const unsigned char* row = st[j] + key * pitch + t * 4 * NW + 4 * w;
-                            const uint4* turn = sm.turn[(j == 0 ? in_macro : in_second) * kUnit + key];
+                            const uint4* turn = sm.turn[(j == 0 ? in_macro : in_second) * kUnit + key_of(g + 8 * r)];
                             const uint4 c4 = turn[(4 * w + t) ^ swap], s4 = turn[(4 * (NW + w) + t) ^ swap];
                             const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
                             uint32_t x[4], y[4];
-                            e2m1x8_to_f16(*reinterpret_cast<const uint32_t*>(row), x);
-                            e2m1x8_to_f16(*reinterpret_cast<const uint32_t*>(row + D / 4), y);
+                            e2m1x8_to_f16(k_lo[j][r][w], x);
+                            e2m1x8_to_f16(k_hi[j][r][w], y);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const uint32_t xs = mul2(x[e], s_lo[j][r]), ys = mul2(y[e], s_hi[j][r]);
@@ -692,11 +740,6 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
         }
         u0 = u1;
     }
-    if (requests && __any_sync(0xffffffffu, dead) && lane < share)       // given up: the copies still have to land (or time out)
-        for (int i = max(before - stages, 0); i < before; ++i) {
-            bool gone = false;
-            wait_phase(smem_u32(&sm.full[lane][i % stages]), i / stages & 1, p.status, gone);
-        }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -808,6 +851,13 @@ cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
     static SmemConfig configured = {};
     p.share = shares_of<D>((p.hkv + tc_head_blocks(p.hkv) - 1) / tc_head_blocks(p.hkv));
     p.step_units = 2 * p.share;
+    // The computing warpgroups wait for registers that the launch has to have brought along: never launch without them.
+    static const bool enough = [] {
+        cudaFuncAttributes attr;
+        return cudaFuncGetAttributes(&attr, quant_attend_tc_kernel<D, CAP, PIECE>) == cudaSuccess &&
+               attr.numRegs * kQtThreads >= kQtComputeRegs * 32 * kQtWarps + kQtLoadRegs * 32 * kQtLoaders;
+    }();
+    if (!enough) return cudaErrorInvalidDeviceFunction;
     cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP, PIECE>, kQtBytes, configured);
     if (e != cudaSuccess) return e;
     e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), kQtBytes, stream, p);
