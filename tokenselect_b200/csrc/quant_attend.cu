@@ -232,8 +232,12 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 // ------------------------------------------------------------------------------------------------
 // Tensor cores: bf16
 // ------------------------------------------------------------------------------------------------
-// What bounds it: HBM in the long run (144 bytes a row and head for 512 a group-of-four bf16 flops), and close behind it the
-// instructions that turn 4-bit codes into operands; so the layout spares those.
+// What bounds it: the instructions that turn 4-bit codes into operands.  A unit of sixteen rows of one head is 2304 bytes, at
+// the copy rate 395 cycles of a scheduler; its 128 conversions, scalings and turns a lane, 16 products and the rest are 506
+// instructions, and take about 750 (2.7 TB/s of 6.55: 4 requests of 100000..262144 tokens, 28 heads over 4).  So the layout
+// spares instructions.  (On the way, the same case: rows in 16-byte cp.async pieces by the computing warps 175 us, bulk copies by
+// one requesting warp 420, by four in turn 166; a partial result per warp instead of per CTA 158; shared memory free of bank
+// conflicts 150.)
 //
 // A warp takes one KV head; its up to eight query heads are the N of m16n8k16 products in fp16.  S^T = K Q^T has sixteen
 // keys as M: a key row's codes, read eight bytes at a time, ARE the A fragments of a thread once converted, because a
@@ -250,9 +254,10 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 // Rows arrive through rings in shared memory: the warps that take the same units (one per KV head) share one.  Four warps of
 // their own request the units in turn, all heads of the CTA at once.  With three heads or more that is one bulk copy a row,
 // sixteen by one instruction, which holds its warp for a microsecond whatever their number and size (measured, random rows, four
-// warps: 6.4 TB/s in rows of 1152 bytes, 4.2 in rows of 576, but 1.1 in rows of 144).  Narrower rows, and rows of D = 64 that lie off the
-// copies' 16-byte grid, come in cp.async pieces.  A row takes 16 bytes modulo 128 in shared memory, and the order in which
-// the sixteen keys are given to the sixteen M rows then makes every read of eight-byte fragments free of bank conflicts.
+// warps: 6.4 TB/s in rows of 1152 bytes, 4.2 in rows of 576, but 1.1 in rows of 144).  Narrower rows, and rows of D = 64 that
+// lie off the copies' 16-byte grid, come in cp.async pieces.  (1.2 million rows of one head: pieces 155 us, bulk 192; 300000
+// rows of two: 56 and 65; 800000 rows of four: 177 and 174.)  A row takes 16 bytes modulo 128 in shared memory, and the order in
+// which the sixteen keys are given to the sixteen M rows then makes every read of eight-byte fragments free of bank conflicts.
 // Eight computing warps with their operands in registers do as well as sixteen with some of them spilled.
 constexpr int kQtWarps = 8, kQtLoaders = 4, kQtThreads = 32 * (kQtWarps + kQtLoaders);
 constexpr int kQtBulkBytes = 400;                              // bulk copies for rows of at least this many
@@ -721,8 +726,8 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                 l1 += __shfl_xor_sync(0xffffffffu, l1, off);
             }
         }
-        // This warp's partial result.  Elements of a head in the order in which the lanes hold them (element_at), so that eight
-        // lanes' pairs are 64 bytes side by side.
+        // This warp's partial result.  Elements of a head in the order in which the lanes hold them, so that eight lanes'
+        // pairs are 64 bytes side by side; the join puts them back.
         if (busy) {
             const long long slot = (long long)(blockIdx.x + b) * share + my_share;
 #pragma unroll
