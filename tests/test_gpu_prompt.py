@@ -151,6 +151,44 @@ def test_what_is_not_finite_reaches_only_the_tokens_that_attend_to_it(bad, dtype
             assert not bool(torch.isfinite(out.cpu()[touched][:, 5]).any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_an_infinite_value_of_the_next_sequence_or_of_a_later_token(dtype):
+    """The block of keys at a sequence's end holds the next sequence's first values, the one on the diagonal those of later
+    tokens: neither reaches a token that does not attend to them, and a long run of undefined values keeps the call's waits."""
+    lens, hq, hkv, d = [200, 700, 3], 4, 2, 128
+    q, k, v, cu = _prompt_case(31, hq, hkv, d, lens, dtype)
+    good = prompt.prompt_attend(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), 0.1)
+    tol = 1e-5 if dtype == F32 else 2.0 ** -7 * 8
+    for first, last in ((200, 201), (900, 903), (250, 900), (0, 1)):
+        v2 = v.clone()
+        v2[first:last] = float("inf")
+        v2[first:last, :, ::2] = float("nan")
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = prompt.prompt_attend(q.cuda(), k.cuda(), v2.cuda(), cu.cuda(), 0.1, status=status).cpu()
+        clean = torch.ones(903, dtype=torch.bool)
+        for a, n in ((0, 200), (200, 700), (900, 3)):
+            if a <= first < a + n:
+                clean[first:a + n] = False
+        assert int(status) == 0 and bool(torch.isfinite(out[clean]).all())
+        assert (out[clean].float() - good.cpu()[clean].float()).abs().max() <= tol
+        assert not bool(torch.isfinite(out[~clean]).any())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_maxima_that_jump(dtype):
+    """A key whose logit is far above all before it, by what O follows (2^55), and by more than it could hold (2^700); at the
+    start, inside and at the end of a block of keys."""
+    n, hq, hkv, d, scale = 600, 2, 1, 128, 0.5
+    q, k, v, cu = _prompt_case(37, hq, hkv, d, [n], F32)
+    u = torch.randn(d, generator=torch.Generator().manual_seed(3))
+    u *= 11.3137 / u.norm()                                                   # |u|^2 = 128
+    q = (u + 0.1 * q).to(dtype)
+    for at, factor in ((150, 0.6), (128, 8.0), (255, 8.0), (40, 8.0), (383, 0.6)):
+        k2 = 0.05 * k
+        k2[at] = u * factor
+        _check_prompt(q, k2.to(dtype), v.to(dtype), cu, [n], scale)
+
+
 def test_slices_of_a_projection_and_other_strides():
     hq, hkv, d, lens = 4, 2, 128, [77, 200]
     n = sum(lens)
@@ -173,6 +211,26 @@ def test_bounds_that_make_no_sense_are_reported():
         out = torch.full_like(args[0].to(dtype), 3.0)
         prompt.prompt_attend(*[t.to(dtype) for t in args], torch.zeros(1, dtype=torch.int32, device="cuda"), 0.1, out=out)
         assert bool((out == 3.0).all())
+
+
+def test_offsets_beyond_31_bits():
+    """The last tokens of tensors of more than 2^31 elements."""
+    t, hq, hkv, d, n = 530000, 32, 1, 128, 100
+    assert t * hq * d > 1 << 31
+    small = _prompt_case(41, hq, hkv, d, [n], BF16)
+    big = []
+    for x in small[:3]:
+        y = torch.empty(t, x.shape[1], d, dtype=BF16, device="cuda")
+        y[-n:] = x.cuda()
+        big.append(y)
+    cu = torch.tensor([t - n, t], dtype=torch.int32, device="cuda")
+    out = prompt.prompt_attend(*big, cu, 0.1)[-n:]
+    assert torch.equal(out, prompt.prompt_attend(*[x.cuda() for x in small[:3]], small[3].cuda(), 0.1))
+    pos = torch.arange(t, dtype=torch.int32, device="cuda")
+    a, b = prompt.norm_rotate(big[0], big[1], pos, 5e5, q_out=big[0], k_out=big[1])
+    wq = ref.rotate(small[0][-2:], pos[-2:].cpu(), 5e5)
+    _near(a[-2:], wq, _norm_tol(wq, small[0][-2:].double(), BF16))
+    assert torch.equal(b[-n:], prompt.norm_rotate(small[0].cuda(), small[1].cuda(), pos[-n:].contiguous(), 5e5)[1])
 
 
 def test_prompt_attention_in_graphs_and_on_streams():

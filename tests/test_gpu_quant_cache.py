@@ -194,7 +194,8 @@ def _check_attend(case, hq, sm_scale, base, **kw):
 @pytest.mark.parametrize("hq,hkv,d,lens", [
     (32, 8, 128, [1]), (32, 8, 128, [700]), (28, 4, 128, [1, 2, 15, 16, 17, 31, 33, 64, 65, 127, 300]), (8, 1, 128, [129, 0, 1000]),
     (7, 1, 128, [513]), (4, 4, 128, [77, 200]), (6, 3, 128, [40, 5]), (8, 2, 64, [1, 16, 100, 333]), (3, 3, 64, [18]), (5, 1, 64, [64, 0, 0, 63]),
-    (16, 16, 128, [90]), (40, 20, 64, [50, 3]),
+    (16, 16, 128, [90]), (40, 20, 64, [50, 3]), (9, 9, 64, [70, 5]), (11, 11, 128, [40, 90]), (12, 6, 64, [100]), (8, 1, 128, [3000, 17]),
+    (5, 1, 64, [2500]), (14, 2, 128, [1500, 0, 700]),
 ], ids=str)
 def test_attention_over_a_4bit_pool(hq, hkv, d, lens, dtype):
     _check_attend(_attend_case(hq + d + len(lens), hq, hkv, d, lens, dtype), hq, d ** -0.5, 5e5)

@@ -277,6 +277,7 @@ struct PromptTcSmem {
     uint64_t q_full, q_empty, kv_full[kPtStages], kv_empty[kPtStages], s_full[2], p_full[2][2], o_full[2], o_empty[2];
     uint64_t queue_full[kPtQueue], queue_empty[kPtQueue], drained;
     uint32_t tmem;
+    int slow;                                                  // warps that compute rows again
 };
 
 // Blocks of keys that half h of a tile sees; 0 when the sequence ends before it.
@@ -377,6 +378,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     PromptTcSmem<D>& sm = *reinterpret_cast<PromptTcSmem<D>*>(dyn + ((1024u - (smem_u32(dyn) & 1023u)) & 1023u));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        sm.slow = 0;
         mbar_init(smem_u32(&sm.q_full), 1);
         mbar_init(smem_u32(&sm.q_empty), 1);
         mbar_init(smem_u32(&sm.drained), 1);
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     int taken = 0;
     auto next_tile = [&]() {
         const int i = taken % kPtQueue;
-        wait_phase(smem_u32(&sm.queue_full[i]), taken / kPtQueue & 1, p.status, dead);
+        wait_phase(smem_u32(&sm.queue_full[i]), taken / kPtQueue & 1, p.status, dead, &sm.slow);
         dead = __any_sync(0xffffffffu, dead);                  // a warp gives up as one
         const int4 t = dead ? make_int4(0, -1, 0, 0) : sm.queue[i];
         __syncwarp();
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 t = make_int4(seq.x, seq.y, order.level, head);
             }
             const int i = put % kPtQueue;
-            wait_phase(smem_u32(&sm.queue_empty[i]), (put / kPtQueue & 1) ^ 1, p.status, dead);
+            wait_phase(smem_u32(&sm.queue_empty[i]), (put / kPtQueue & 1) ^ 1, p.status, dead, &sm.slow);
             dead = __any_sync(0xffffffffu, dead);
             if (dead) t.y = -1;
             __syncwarp();
@@ -449,14 +451,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             if (t.y < 0) break;
             const int n0 = blocks_of(t.y, t.z, 0), n1 = blocks_of(t.y, t.z, 1), n = max(n0, n1);
             if (lane == 0) {
-                wait_phase(smem_u32(&sm.q_empty), (put & 1) ^ 1, p.status, dead);
+                wait_phase(smem_u32(&sm.q_empty), (put & 1) ^ 1, p.status, dead, &sm.slow);
                 mbar_expect_tx(smem_u32(&sm.q_full), n1 > 0 ? 2 * kTile : kTile);
                 for (int h = 0; h < (n1 > 0 ? 2 : 1); ++h)
                     for (int c = 0; c < kParts; ++c)
                         tile_g2s(smem_u32(sm.q[h]) + c * kPart, &map_q, 64 * c, t.w, t.x + t.z * 2 * kPtRows + h * kPtRows, smem_u32(&sm.q_full));
                 for (int j = 0; j < 2 * n; ++j, ++kv) {        // K_0, V_0, K_1, ...
                     const int s = kv % kPtStages;
-                    wait_phase(smem_u32(&sm.kv_empty[s]), (kv / kPtStages & 1) ^ 1, p.status, dead);
+                    wait_phase(smem_u32(&sm.kv_empty[s]), (kv / kPtStages & 1) ^ 1, p.status, dead, &sm.slow);
                     mbar_expect_tx(smem_u32(&sm.kv_full[s]), kTile);
                     for (int c = 0; c < kParts; ++c)
                         tile_g2s(smem_u32(sm.kv[s]) + c * kPart, j & 1 ? &map_v : &map_k, 64 * c, t.w / p.group, t.x + (j >> 1) * kPtBlock, smem_u32(&sm.kv_full[s]));
@@ -468,10 +470,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         if (lane == 0 && dead) {                               // given up: the copies still have to land (or time out)
             for (int i = max(kv - kPtStages, 0); i < kv; ++i) {
                 bool gone = false;
-                wait_phase(smem_u32(&sm.kv_full[i % kPtStages]), i / kPtStages & 1, p.status, gone);
+                wait_phase(smem_u32(&sm.kv_full[i % kPtStages]), i / kPtStages & 1, p.status, gone, &sm.slow);
             }
             bool gone = false;
-            if (put > 0) wait_phase(smem_u32(&sm.q_full), (put - 1) & 1, p.status, gone);
+            if (put > 0) wait_phase(smem_u32(&sm.q_full), (put - 1) & 1, p.status, gone, &sm.slow);
         }
         __syncwarp();
     } else if (warp == 8) {
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             if (elect_one()) {
                 auto wait_block = [&](int i) {                 // block i of the tile's K_0, V_0, K_1, ...
                     const int s = (kv + i) % kPtStages;
-                    wait_phase(smem_u32(&sm.kv_full[s]), (kv + i) / kPtStages & 1, p.status, dead);
+                    wait_phase(smem_u32(&sm.kv_full[s]), (kv + i) / kPtStages & 1, p.status, dead, &sm.slow);
                     tcgen05_after_sync();
                     return smem_u32(sm.kv[s]);
                 };
@@ -506,14 +508,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {           // 16 keys a step: 8 columns of P, which comes in two parts
                         if (ks % 4 == 0) {
-                            wait_phase(smem_u32(&sm.p_full[h][ks / 4]), p_count[h] & 1, p.status, dead);
+                            wait_phase(smem_u32(&sm.p_full[h][ks / 4]), p_count[h] & 1, p.status, dead, &sm.slow);
                             tcgen05_after_sync();
                         }
                         mma_ts(tmem + kO + 128u * h, tmem + 128u * h + 8u * ks, sw128_operand(v + ks * 2048u, kPart, 1024), kIdescPV, !first || ks > 0 ? 1u : 0u);
                     }
                     ++p_count[h];
                 };
-                wait_phase(smem_u32(&sm.q_full), tiles & 1, p.status, dead);
+                wait_phase(smem_u32(&sm.q_full), tiles & 1, p.status, dead, &sm.slow);
                 uint32_t k = wait_block(0);
                 issue_qk(0, k);
                 if (n_of[1] > 0) issue_qk(1, k);
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     for (int h = 0; h < 2; ++h) {
                         if (j < n_of[h]) {
                             if (j == 0) {                      // the half's last result has been read
-                                wait_phase(smem_u32(&sm.o_empty[h]), (o_count[h] & 1) ^ 1, p.status, dead);
+                                wait_phase(smem_u32(&sm.o_empty[h]), (o_count[h] & 1) ^ 1, p.status, dead, &sm.slow);
                                 ++o_count[h];
                             }
                             issue_pv(h, v, j == 0);
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         if (lane == 0 && dead) {                               // given up: the products still have to end (or time out)
             bool gone = false;
             mma_commit(smem_u32(&sm.drained));
-            wait_phase(smem_u32(&sm.drained), 0, p.status, gone);
+            wait_phase(smem_u32(&sm.drained), 0, p.status, gone, &sm.slow);
         }
         __syncwarp();
     } else {
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 }
             };
             for (int j = 0; j < n; ++j) {
-                wait_phase(smem_u32(&sm.s_full[h]), s_count & 1, p.status, dead);
+                wait_phase(smem_u32(&sm.s_full[h]), s_count & 1, p.status, dead, &sm.slow);
                 ++s_count;
                 tcgen05_after_sync();
                 // The blocks before raised a row's maximum by more than 2^8: O (every P.V so far is complete) and the sum follow.
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             sum += sum1;
             if (top_x > ref + 100.f) sum = __int_as_float(0x7fc00000);
             // the result
-            wait_phase(smem_u32(&sm.o_full[h]), o_count & 1, p.status, dead);
+            wait_phase(smem_u32(&sm.o_full[h]), o_count & 1, p.status, dead, &sm.slow);
             ++o_count;
             tcgen05_after_sync();
             const float inv = 1.f / sum;
@@ -678,7 +680,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.o_empty[h]));
             unsigned again = __ballot_sync(0xffffffffu, row < t.y && top >= 0x7f800000u);
-            for (; again != 0; again &= again - 1) prompt_row<D>(p, t.x, row - lane + __ffs(again) - 1, t.w);
+            if (again != 0) {                                  // (row by row: the other warps' waits have to be patient)
+                if (lane == 0) atomicAdd(&sm.slow, 1);
+                for (; again != 0; again &= again - 1) prompt_row<D>(p, t.x, row - lane + __ffs(again) - 1, t.w);
+                __syncwarp();
+                if (lane == 0) atomicSub(&sm.slow, 1);
+            }
         }
     }
     tcgen05_before_sync();

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
 #pragma unroll
                 for (int i = 0; i < kQtWarps / 2; ++i)
                     if (mine && w >> 1 == i) {
-                        if (some) ahead[i] = __ldg(table + r); else ahead[i] = INT_MIN;
+                        if (some) ahead[i] = __ldcg(table + r); else ahead[i] = INT_MIN;
                     }
             };
             {

@@ -125,12 +125,15 @@ __device__ __forceinline__ bool test_phase(uint32_t bar, uint32_t parity) {
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// A wait of at most about a second; then the call's status says so, and the waits that follow give up at once.
-__device__ __forceinline__ void wait_phase(uint32_t bar, uint32_t parity, int* status, bool& dead) {
+// A wait of at most about a second; then the call's status says so, and the waits that follow give up at once.  While
+// *`slow` is not 0 (a warp of the CTA is at work that may take long) the time does not run.
+__device__ __forceinline__ void wait_phase(uint32_t bar, uint32_t parity, int* status, bool& dead, const volatile int* slow = nullptr) {
     if (mbar_try_wait(bar, parity) || dead) return;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
+    long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (slow != nullptr && *slow != 0) t0 = clock64();
         if (clock64() - t0 > kWaitCycles) { report(status, TS_ERR_DEVICE_TIMEOUT); dead = true; return; }
+    }
 }
 
 inline bool power_of_two(float g) {
