@@ -748,13 +748,15 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
 }
 
 // ------------------------------------------------------------------------------------------------
-// Join the partial results: grid (hq, batch); a warp has eight of them in flight, so that 128 are one round trip
+// Join the partial results: grid (hq, batch)
 // ------------------------------------------------------------------------------------------------
-constexpr int kQmThreads = 512;
-// LANES: elements in the order of the tensor-core kernel's lanes.
-template <typename T, int D, bool LANES>
-__global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_constant__ QuantAttendParams p) {
-    constexpr int VEC = D / 32, NW = kQmThreads / 32, kAhead = 8;
+// LANES: elements in the order of the tensor-core kernel's lanes.  WARPS, AHEAD: partial results in flight, so that a request's
+// are one round trip: 16 x 10 where a request has many (1 x 131072, 32 heads, the whole call: 61.4 us, 64.5 with 8 x 8), 8 x 8
+// where it has 64 at most on average (16 x 1000..32000, 28 heads: 46.1 us; 52.0 with 16 x 10, whose one CTA per SM makes the 448
+// of them four rounds; 47.6 with 4 x 8).
+template <typename T, int D, bool LANES, int WARPS, int AHEAD>
+__global__ void __launch_bounds__(32 * WARPS) quant_merge_kernel(const __grid_constant__ QuantAttendParams p) {
+    constexpr int VEC = D / 32, NW = WARPS, kAhead = AHEAD;
     __shared__ int start[kQaMaxBatch + 1];
     __shared__ float s_acc[NW][D];
     __shared__ float2 s_ml[NW];
@@ -812,7 +814,7 @@ __global__ void __launch_bounds__(kQmThreads) quant_merge_kernel(const __grid_co
     for (int v = 0; v < VEC; ++v) s_acc[warp][VEC * lane + v] = acc[v];
     if (lane == 0) s_ml[warp] = make_float2(m, l);
     __syncthreads();
-    for (int e = threadIdx.x; e < D; e += kQmThreads) {
+    for (int e = threadIdx.x; e < D; e += 32 * WARPS) {
         float mm = -INFINITY, r = 0.f, ll = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) mm = fmaxf(mm, s_ml[w].x);
@@ -844,12 +846,18 @@ size_t partial_slots(int sms, int batch, int hq) {
 }
 size_t partial_bytes(int sms, int batch, int hq, int d) { return partial_slots(sms, batch, hq) * hq * (d + 2) * sizeof(float); }
 
+template <typename T, int D, bool LANES>
+cudaError_t launch_merge(const QuantAttendParams& p, cudaStream_t stream) {
+    const dim3 grid(p.hq, p.batch);
+    return p.pieces * p.share / p.batch > 64 ? launch_chained(quant_merge_kernel<T, D, LANES, 16, 10>, grid, dim3(512), 0, stream, p)
+                                             : launch_chained(quant_merge_kernel<T, D, LANES, 8, 8>, grid, dim3(256), 0, stream, p);
+}
 template <int D>
 cudaError_t launch_attend_plain(const QuantAttendParams& p, cudaStream_t stream) {
     const int nsub = (p.group + kQpHeads - 1) / kQpHeads, per_cta = kQpThreads / 32;
     const cudaError_t e = launch_chained(quant_attend_plain_kernel<float, D>, dim3(p.pieces, (p.hkv * nsub + per_cta - 1) / per_cta), dim3(kQpThreads), 0, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_chained(quant_merge_kernel<float, D, false>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+    return launch_merge<float, D, false>(p, stream);
 }
 template <int D, bool CAP, int PIECE>
 cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
@@ -867,7 +875,7 @@ cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), kQtBytes, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_chained(quant_merge_kernel<__nv_bfloat16, D, true>, dim3(p.hq, p.batch), dim3(kQmThreads), 0, stream, p);
+    return launch_merge<__nv_bfloat16, D, true>(p, stream);
 }
 template <int D, bool CAP>
 cudaError_t launch_attend_bf16(const QuantAttendParams& p, cudaStream_t stream) {
