@@ -212,6 +212,13 @@ def test_attention_of_a_long_request_and_many_short_ones():
     _check_attend(_attend_case(21, 8, 2, 128, [9000] + [(7 * i) % 23 for i in range(300)], BF16), 8, 128 ** -0.5, 5e5)
 
 
+@pytest.mark.parametrize("hq,hkv,d,lens", [(2, 1, 128, [150000]), (4, 2, 128, [70000, 50001]), (4, 2, 64, [110000]), (5, 5, 64, [60000]),
+                                           (6, 3, 128, [40000, 40007])])
+def test_rings_of_every_width_go_round(hq, hkv, d, lens):
+    """Enough rows that every CTA fills its stages several times, however many a row's width leaves room for."""
+    _check_attend(_attend_case(25, hq, hkv, d, lens, BF16), hq, d ** -0.5, 5e5)
+
+
 def test_queries_of_any_size_and_alignment():
     """fp16 holds the rotated query whatever its size: it is scaled by a power of two."""
     case = list(_attend_case(31, 8, 2, 128, [100, 40], BF16))

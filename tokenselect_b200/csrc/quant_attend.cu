@@ -251,19 +251,29 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 // exact distance to the tile's first key, and a key only by its place i in the tile, from a table of 128 rows of cosines and
 // sines in fp16 that stays in shared memory.  No table grows with the context, and the far angles stay exact.
 //
-// Rows arrive through rings in shared memory: the warps that take the same units (one per KV head) share one.  Four warps of
+// Rows arrive through rings in shared memory: the warps that take the same units (one per KV head) share one.  Warps of
 // their own request the units in turn, all heads of the CTA at once.  With three heads or more that is one bulk copy a row,
 // sixteen by one instruction, which holds its warp for a microsecond whatever their number and size (measured, random rows, four
 // warps: 6.4 TB/s in rows of 1152 bytes, 4.2 in rows of 576, but 1.1 in rows of 144).  Narrower rows, and rows of D = 64 that
-// lie off the copies' 16-byte grid, come in cp.async pieces.  (1.2 million rows of one head: pieces 155 us, bulk 192; 300000
-// rows of two: 56 and 65; 800000 rows of four: 177 and 174.)  A row takes 16 bytes modulo 128 in shared memory, and the order in
+// lie off the copies' 16-byte grid, come in cp.async pieces.  (1.2 million rows of one head: pieces 107 us, bulk 192; 300000
+// rows of two: 51 and 64; 800000 rows of four: 187 and 174.)  A row takes 16 bytes modulo 128 in shared memory, and the order in
 // which the sixteen keys are given to the sixteen M rows then makes every read of eight-byte fragments free of bank conflicts.
 // Eight computing warps with their operands in registers do as well as sixteen with some of them spilled.
-constexpr int kQtWarps = 8, kQtLoaders = 4, kQtThreads = 32 * (kQtWarps + kQtLoaders);
+constexpr int kQtWarps = 8;
 constexpr int kQtBulkBytes = 400;                              // bulk copies for rows of at least this many
-constexpr int kQtComputeRegs = 224, kQtLoadRegs = 56;          // of a launch with 168 a thread: 2 * 224 + 56 = 3 * 168
+constexpr int kQtLoadRegs = 56;
+// Requesting warps, and registers: those they give up are the computing ones'.  Four for bulk copies; eight for rows in pieces, of
+// which a warp has few in flight (1.2 million rows of one head: 153 us with four, 106 with eight; bulk rows of eight heads 123 and
+// 133, because the computing warps then get 200 registers).
+template <int PIECE>
+struct QtLaunch {
+    static constexpr int kLoaders = PIECE == 0 ? 4 : 8, kThreads = 32 * (kQtWarps + kLoaders);
+    static constexpr int kComputeRegs = PIECE == 0 ? 224 : 200;        // 2 * 224 + 56 = 3 * 168; 2 * 200 + 2 * 56 = 4 * 128 a thread
+};
 constexpr int kQtMacro = 8;                                    // units of a macro tile
-// Stages of a ring: a step holds two while the two behind it arrive, so fewer than four would wait for themselves.
+// Stages of a ring: a step holds two while the two behind it arrive, so fewer than four would wait for themselves.  And never
+// fewer than warps that fill it in turn: a warp asks for the stage's release before last with the same parity, and knows that one
+// to have happened because it filled a stage that many units ago.
 constexpr int kQtMinStages = 4, kQtMaxStages = 8, kQtBytes = 232448;          // (dynamic shared memory)
 
 template <int D>
@@ -360,8 +370,9 @@ __device__ __forceinline__ Segment segment_at(const QuantAttendParams& p, const 
 
 // PIECE: 0, rows by bulk copies; 16 or 8, by pieces of that many bytes.
 template <int D, bool CAP, int PIECE>
-__global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __grid_constant__ QuantAttendParams p) {
+__global__ void __launch_bounds__(QtLaunch<PIECE>::kThreads, 1) quant_attend_tc_kernel(const __grid_constant__ QuantAttendParams p) {
     using Row = QuantRow<D>;
+    using Launch = QtLaunch<PIECE>;
     constexpr int HALF = D / 2, NW = D / 64, MT = D / 16;      // words a half, M tiles of O
     extern __shared__ __align__(16) unsigned char dyn[];
     QuantTcSmem<D>& sm = *reinterpret_cast<QuantTcSmem<D>*>(dyn);
@@ -373,7 +384,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
     {
         const int pair = threadIdx.x % HALF, owner = pair / (D / 8), r = pair % (D / 8);
         const unsigned long long f = p.freqs.f[pair];
-        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit; i += kQtThreads / HALF) {
+        for (int i = threadIdx.x / HALF; i < kQtMacro * kUnit; i += Launch::kThreads / HALF) {
             const float2 cs = cos_sin_fast(i, f);
             __half* row = reinterpret_cast<__half*>(sm.turn[i]);
             const int swap = (i & 2) * 2;
@@ -416,6 +427,9 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
         // ---------------- requests ----------------
         // (these warps leave their registers to the computing ones)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kQtLoadRegs));
+        static_assert(kQtMinStages >= QtLaunch<0>::kLoaders, "stages for the warps of bulk copies");
+        const int turns = PIECE == 0 ? Launch::kLoaders : min(Launch::kLoaders, stages), my_turn = warp - kQtWarps;
+        if (my_turn >= turns) return;
         int before = 0;                                        // lane w: units of share w in the segments so far
         while (u0 < u_end) {
             const Segment seg = segment_at(p, sm.start, u0, u_end, share);
@@ -423,10 +437,10 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
             const int* table = seg.table;
             auto units_of = [&](int w) { return seg.units_of(u0, w, share); };
             // Lane w keeps the place of share w: unit `at` of its units, counted over all requests, goes into stage at % stages and is
-            // requested by warp at % 4 of these.  Lanes 16 (w & 1) + r of ahead[w / 2] hold the number of row r of this warp's next
+            // requested by warp at % turns of these.  Lanes 16 (w & 1) + r of ahead[w / 2] hold the number of row r of this warp's next
             // unit (or none), read when the one before was requested.
             const int end = before + (lane < share ? units_of(lane) : 0);
-            int at = before + ((warp - kQtWarps - before) & (kQtLoaders - 1)), ahead[kQtWarps / 2];
+            int at = before + (my_turn + turns - before % turns) % turns, ahead[kQtWarps / 2];
             auto unit_of = [&]() { const int k = at - before, m = k / per; return u0 + (m * share + lane) * per + k - m * per; };
             auto read_ahead = [&](int w, int unit) {
                 const int r = (unit - first) * kUnit + (lane & 15);
@@ -481,7 +495,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
                         for (int j = (lane >> 4) * PIECE; j < width; j += 2 * PIECE) copy_piece<PIECE>(smem_u32(dst + r * pitch + j), src + (some ? j : 0), some ? PIECE : 0);
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
                     }
-                    if (lane == w) at += kQtLoaders;
+                    if (lane == w) at += turns;
                     const int unit = unit_of();
                     read_ahead(w, __shfl_sync(0xffffffffu, unit, w));
                 }
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quant_attend_tc_kernel(const __
         return;
     }
     // ---------------- products ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kQtComputeRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Launch::kComputeRegs));
     int stage = 0;                                             // next stage to read
     uint32_t phase = 0;                                        // parity of its barrier
     while (u0 < u_end) {
@@ -861,6 +875,7 @@ cudaError_t launch_attend_plain(const QuantAttendParams& p, cudaStream_t stream)
 }
 template <int D, bool CAP, int PIECE>
 cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
+    using Launch = QtLaunch<PIECE>;
     static SmemConfig configured = {};
     p.share = shares_of<D>((p.hkv + tc_head_blocks(p.hkv) - 1) / tc_head_blocks(p.hkv));
     p.step_units = 2 * p.share;
@@ -868,12 +883,12 @@ cudaError_t launch_attend_tc(QuantAttendParams p, cudaStream_t stream) {
     static const bool enough = [] {
         cudaFuncAttributes attr;
         return cudaFuncGetAttributes(&attr, quant_attend_tc_kernel<D, CAP, PIECE>) == cudaSuccess &&
-               attr.numRegs * kQtThreads >= kQtComputeRegs * 32 * kQtWarps + kQtLoadRegs * 32 * kQtLoaders;
+               attr.numRegs * Launch::kThreads >= Launch::kComputeRegs * 32 * kQtWarps + kQtLoadRegs * 32 * Launch::kLoaders;
     }();
     if (!enough) return cudaErrorInvalidDeviceFunction;
     cudaError_t e = ensure_dynamic_smem(quant_attend_tc_kernel<D, CAP, PIECE>, kQtBytes, configured);
     if (e != cudaSuccess) return e;
-    e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(kQtThreads), kQtBytes, stream, p);
+    e = launch_chained(quant_attend_tc_kernel<D, CAP, PIECE>, dim3(p.pieces, tc_head_blocks(p.hkv)), dim3(Launch::kThreads), kQtBytes, stream, p);
     if (e != cudaSuccess) return e;
     return launch_merge<__nv_bfloat16, D, true>(p, stream);
 }
