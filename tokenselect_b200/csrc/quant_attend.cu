@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(kQpThreads) quant_attend_plain_kernel(const __
 // lie off the copies' 16-byte grid, come in cp.async pieces.  (1.2 million rows of one head: pieces 107 us, bulk 192; 300000
 // rows of two: 51 and 64; 800000 rows of four: 187 and 174.)  A row takes 16 bytes modulo 128 in shared memory, and the order in
 // which the sixteen keys are given to the sixteen M rows then makes every read of eight-byte fragments free of bank conflicts.
-// Eight computing warps with their operands in registers do as well as sixteen with some of them spilled.
+// Eight computing warps with their operands in registers do as well as sixteen with some of them spilled, and better than twelve
+// in 152 registers (4 x 200000, 28 heads over 4: 173 and 184 us).
 constexpr int kQtWarps = 8;
 constexpr int kQtBulkBytes = 400;                              // bulk copies for rows of at least this many
 constexpr int kQtLoadRegs = 56;
