@@ -304,3 +304,43 @@ def test_prompts_and_decode_steps_over_a_4bit_cache(d):
             pair = (kh.abs() + kh.abs().roll(d // 2, -1))[:, torch.arange(hq) // (hq // hkv)]
             e = 6 * 5 * 2.0 ** -11 * scale * ((qq * pair) ** 2).sum(-1).sqrt().amax(0)
             _near(out[b].view(1, hq, d), o, 2.0 ** -8 * o.abs() + (torch.exp(2 * e)[:, None] - 1 + 2.0 ** -10) * m)
+
+
+def _matches(out, want, mag):
+    """Finite where the 64-bit form is, and near it there."""
+    out, fine = out.cpu().double(), torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), fine), f"{int((torch.isfinite(out) != fine).sum())} elements finite that should not be, or not that should"
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 1e-3) * mag
+    assert bool(((out - want).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("d", [64, 128])
+def test_an_undefined_key_at_any_place_reaches_every_later_token(d, cap):
+    """A NaN in a key makes every token from it on undefined, whatever its place in its block of keys and however many
+    blocks later the token comes; earlier tokens, the other head and the other sequence do not see it."""
+    lens, hq, hkv = [30, 520], 2, 2
+    q, k, v, cu = _prompt_case(43, hq, hkv, d, lens, BF16)
+    for at in (0, 1, 2, 3, 4, 5, 6, 7, 30, 95, 127, 134, 383):
+        k2 = k.clone()
+        k2[30 + at, 1, at % d] = float("nan")
+        out = prompt.prompt_attend(q.cuda(), k2.cuda(), v.cuda(), cu.cuda(), 0.1, cap).cpu()
+        seen = torch.zeros(550, hq, dtype=torch.bool)
+        seen[30 + at:, 1] = True
+        assert bool(torch.isfinite(out[~seen]).all()), at
+        assert not bool(torch.isfinite(out[seen]).any()), (at, int(torch.isfinite(out[seen]).sum()))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinite_keys_give_what_the_softmax_gives(d):
+    """An infinite key gives a logit of plus infinity (the softmax is undefined), of minus infinity (a weight of zero) or, where
+    two infinities meet, none; a token all of whose logits are minus infinity has no softmax either."""
+    n, hq, hkv = 400, 2, 1
+    q, k, v, cu = _prompt_case(47, hq, hkv, d, [n], BF16)
+    one, two, all_ = k.clone(), k.clone(), k.clone()
+    one[6, 0, 5] = float("inf")
+    two[7, 0, 5], two[7, 0, 6] = float("inf"), -float("inf")
+    all_[:, 0, 5] = -float("inf")
+    for k2 in (one, two, all_):
+        out = prompt.prompt_attend(q.cuda(), k2.cuda(), v.cuda(), cu.cuda(), d ** -0.5)
+        _matches(out, *ref.attend(q, k2, v, ref.causal([n], n), d ** -0.5))

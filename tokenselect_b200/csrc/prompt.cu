@@ -268,6 +268,7 @@ cudaError_t launch_prompt_plain(const PromptParams& p, cudaStream_t stream) {
 constexpr int kPtRows = 128, kPtBlock = 128;                   // rows of a half, keys of a block
 constexpr int kPtStages = 5, kPtThreads = 320;                 // two times four softmax warps, one that issues products, one that requests tiles
 constexpr int kPtQueue = 2;
+constexpr float kPtLowest = -3e38f;                            // reference of a row none of whose logits is above it
 
 template <int D>
 struct PromptTcSmem {
@@ -342,7 +343,7 @@ __device__ __noinline__ void prompt_row(const PromptParams& p, int first, int ro
     for (int e = 0; e < E; ++e) out[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
 }
 
-// 2^x of two numbers on the multipliers, for x >= -125 (below, 2^-125): 2^n 2^f with n the nearest whole number and 2^f a
+// 2^x of two numbers on the multipliers, for x >= -125 (below, and for minus infinity and NaN, 2^-125): 2^n 2^f with n the nearest whole number and 2^f a
 // polynomial of degree 3 (Remez exchange: 7.5e-5 relative on [-1/2, 1/2], a twentieth of the weight's rounding to bf16).
 __device__ __forceinline__ uint64_t exp2_f32x2(uint64_t x) {
     float a, b;
@@ -358,6 +359,19 @@ __device__ __forceinline__ uint64_t exp2_f32x2(uint64_t x) {
     unpack_f32x2(y, ya, yb);
     unpack_f32x2(n, na, nb);
     return pack_f32x2(__int_as_float(__float_as_int(ya) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(yb) + (__float_as_int(nb) << 23)));
+}
+
+// The largest, and NaN where one of them is: what the multipliers make of an undefined logit is a number like any other, so the
+// maximum is what remembers it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // True for one lane of a converged warp.  (With `lane == 0` in its place the compiler does not know the code behind it to be
@@ -583,18 +597,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                         for (int e = 0; e < 32; ++e)
                             if (32 * c + e > r) y32[e] = -INFINITY;
                     }
-                    float m4[4] = {y32[0], y32[1], y32[2], y32[3]};
+                    float m4[4];
 #pragma unroll
-                    for (int e = 4; e < 32; e += 4)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], y32[e + i]);
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+                    for (int i = 0; i < 4; ++i) {
+                        m4[i] = max_nan(y32[i], y32[4 + i], y32[8 + i]);
+                        m4[i] = max_nan(m4[i], y32[12 + i], y32[16 + i]);
+                        m4[i] = max_nan(m4[i], y32[20 + i], y32[24 + i]);
+                        m4[i] = max_nan(m4[i], y32[28 + i]);
+                    }
+                    const float mx = max_nan(max_nan(m4[0], m4[1], m4[2]), m4[3]) * mul;
                     if (fresh) {                               // any number near the maximum will do: that of the first 32 keys
-                        ref = fmaxf(mx, -1e30f);
+                        ref = fmaxf(mx, kPtLowest);
                         top_x = ref;
                         fresh = false;
                     }
-                    top_x = fmaxf(top_x, mx);
+                    top_x = max_nan(top_x, mx);
                     const uint64_t mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(-ref, -ref);
                     uint32_t w[16];
 #pragma unroll
@@ -651,7 +668,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             float sum, sum1;
             unpack_f32x2(add_f32x2(sums[0], sums[1]), sum, sum1);
             sum += sum1;
-            if (top_x > ref + 100.f) sum = __int_as_float(0x7fc00000);
+            // (an undefined or infinite logit makes the row undefined, and so do logits that are minus infinity without exception)
+            if (!(top_x > kPtLowest && top_x <= fminf(ref + 100.f, 3.4028235e38f))) sum = __int_as_float(0x7fc00000);
             // the result
             wait_phase(smem_u32(&sm.o_full[h]), o_count & 1, p.status, dead, &sm.slow);
             ++o_count;
