@@ -344,3 +344,48 @@ def test_infinite_keys_give_what_the_softmax_gives(d):
     for k2 in (one, two, all_):
         out = prompt.prompt_attend(q.cuda(), k2.cuda(), v.cuda(), cu.cuda(), d ** -0.5)
         _matches(out, *ref.attend(q, k2, v, ref.causal([n], n), d ** -0.5))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_columns_that_become_undefined_one_after_the_other(d):
+    """Values that are not finite, each in a column of its own, in the same block of keys and in later ones, before and behind
+    the tokens of a block, with keys far above the others among them: every column of every token is finite where the tokens
+    it sees are."""
+    lens, hq, hkv = [700, 150], 4, 2
+    q, k, v, cu = _prompt_case(53, hq, hkv, d, lens, BF16)
+    k[260, 0] *= 40.0                                                         # logits that jump for some queries
+    for at, col, x in ((10, 3, "nan"), (300, 7, "inf"), (390, 9, "-inf"), (391, 9, "inf"), (511, 3, "inf"), (512, 40, "nan"), (640, 11, "nan"), (699, 50, "inf"),
+                       (701, 5, "nan"), (849, 6, "inf")):
+        v[at, :, col] = float(x)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = prompt.prompt_attend(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), 0.1, status=status)
+    assert int(status) == 0
+    _matches(out, *ref.attend(q, k, v, ref.causal(lens, 850), 0.1))
+
+
+@pytest.mark.parametrize("columns", [slice(None), slice(5, 6)], ids=["all", "one"])
+def test_an_early_undefined_value_does_not_hold_the_call_up(columns):
+    """An undefined value at the start of a long prompt makes every later token undefined, with cause: no more than a block's
+    tokens are computed again.  (One value after the other on a warp, they would take two hundred times the clean call's time.)"""
+    n, hq, hkv, d = 16384, 8, 1, 128
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda").to(BF16) for h in (hq, hkv, hkv))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    v2 = v.clone()
+    v2[3, :, columns] = float("nan")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    took = []
+    for x in (v, v2):
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = prompt.prompt_attend(q, k, x, cu, d ** -0.5, status=status)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        took.append(min(times))
+    bad = torch.zeros(n, hq, d, dtype=torch.bool, device="cuda")
+    bad[3:, :, columns] = True
+    assert int(status) == 0 and torch.equal(~torch.isfinite(out), bad)
+    assert took[1] <= 10 * took[0], took

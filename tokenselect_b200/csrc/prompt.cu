@@ -263,8 +263,11 @@ cudaError_t launch_prompt_plain(const PromptParams& p, cudaStream_t stream) {
 // last key, longest first, heads innermost (the heads that share K and V run side by side).
 //
 // What is not finite.  A masked weight is 0, but 0 times an infinity in V is not; the block on the diagonal holds the V of
-// later tokens, and of the next sequence.  Only then does a row of O end up non-finite without cause, so rows that do are
-// computed again on the CUDA cores, from the keys that they see (slow, and exact for what is non-finite with cause).
+// later tokens, and of the next sequence.  Only then does a row of O end up non-finite without cause, and mend_rows() has such
+// rows computed again on the CUDA cores, from the keys that they see.  That is slow (150 cycles a key and warp), but few rows: one
+// undefined value at the start of 16384 tokens, 8 heads, 1.0 ms in place of 0.45.  Rows whose logits jump by more than 2^100
+// inside a block are not few where all logits are of that size (the same shape, logits of +-160: 83 ms), so while a warp is
+// at work on rows the clock of its CTA's waits stands still.
 constexpr int kPtRows = 128, kPtBlock = 128;                   // rows of a half, keys of a block
 constexpr int kPtStages = 5, kPtThreads = 320;                 // two times four softmax warps, one that issues products, one that requests tiles
 constexpr int kPtQueue = 2;
@@ -279,6 +282,7 @@ struct PromptTcSmem {
     uint64_t queue_full[kPtQueue], queue_empty[kPtQueue], drained;
     uint32_t tmem;
     int slow;                                                  // warps that compute rows again
+    unsigned jumped[8];                                        // per softmax warp: rows of the tile whose logits jumped
 };
 
 // Blocks of keys that half h of a tile sees; 0 when the sequence ends before it.
@@ -312,35 +316,118 @@ __device__ int sequence_at(const PromptParams& p, int level, int rank) {
     return 0;
 }
 
-// Row `row` of a sequence for one head on the CUDA cores, a warp per row: for rows that met what is not finite.
+// Row `row` of a sequence for one head on the CUDA cores, by one warp: D/8 lanes hold a key's or a value's row, eight elements each,
+// 32 keys a step, of which every lane then has one logit.
 template <int D>
 __device__ __noinline__ void prompt_row(const PromptParams& p, int first, int row, int h) {
-    const int lane = threadIdx.x & 31;
-    constexpr int E = D / 32;
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (long long)(first + row) * p.q_stride + (long long)h * D;
-    const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(p.k) + (long long)first * p.k_stride + (long long)(h / p.group) * D;
-    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v) + (long long)first * p.v_stride + (long long)(h / p.group) * D;
-    float x[E], o[E], m = -INFINITY, l = 0.f;
+    constexpr int kLanes = D / 8, kKeys = 32 / kLanes;         // keys of one load
+    const int lane = threadIdx.x & 31, c = lane % kLanes, g = lane / kLanes;
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (long long)(first + row) * p.q_stride + (long long)h * D + 8 * c;
+    const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(p.k) + (long long)first * p.k_stride + (long long)(h / p.group) * D + 8 * c;
+    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v) + (long long)first * p.v_stride + (long long)(h / p.group) * D + 8 * c;
+    auto floats = [](uint4 a, float (&x)[8]) {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int e = 0; e < E; ++e) { x[e] = __bfloat162float(q[lane + 32 * e]); o[e] = 0.f; }
-    for (int j = 0; j <= row; ++j) {
-        float s = 0.f;
+        for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    };
+    float x[8], y[8], o[8], m = -INFINITY, l = 0.f;
+    floats(*reinterpret_cast<const uint4*>(q), x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += x[e] * __bfloat162float(k[j * p.k_stride + lane + 32 * e]);
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    for (int key0 = 0; key0 <= row; key0 += 32) {
+        float s[kLanes];
 #pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s *= p.sm_scale;
-        if (p.logit_cap > 0.f) s = p.logit_cap * tanhf(s / p.logit_cap);
-        s *= 1.4426950408889634f;
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base), w = exp2f(s - base);
+        for (int i = 0; i < kLanes; ++i) {                     // (behind the row's own key: that one again)
+            floats(*reinterpret_cast<const uint4*>(k + min(key0 + i * kKeys + g, row) * p.k_stride), y);
+            s[i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[i] = fmaf(x[e], y[e], s[i]);
+        }
+        // lane (g, c) ends up with the whole sum of key key0 + c * kKeys + g
+#pragma unroll
+        for (int off = kLanes / 2; off >= 1; off >>= 1) {
+            const bool up = (c & off) != 0;
+#pragma unroll
+            for (int i = 0; i < off; ++i) {
+                const float keep = up ? s[i + off] : s[i], send = up ? s[i] : s[i + off];
+                s[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+            }
+        }
+        float logit = s[0] * p.sm_scale;
+        if (p.logit_cap > 0.f) logit = p.logit_cap * tanhf(logit / p.logit_cap);
+        logit = key0 + c * kKeys + g <= row ? logit * 1.4426950408889634f : -INFINITY;
+        float mn = fmaxf(m, logit);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+        const float base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base), w = exp2f(logit - base);
         m = mn;
         l = l * corr + w;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * corr + w * __bfloat162float(v[j * p.v_stride + lane + 32 * e]);
-    }
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)(first + row) * p.hq + h) * D;
+        for (int e = 0; e < 8; ++e) o[e] *= corr;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
+        for (int i = 0; i < kLanes; ++i) {
+            const int key = key0 + i * kKeys + g;
+            const float wi = __shfl_sync(0xffffffffu, w, g * kLanes + i);
+            const uint4 raw = *reinterpret_cast<const uint4*>(v + min(key, row) * p.v_stride);
+            floats(key <= row ? raw : make_uint4(0u, 0u, 0u, 0u), y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = fmaf(wi, y[e], o[e]);
+        }
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+#pragma unroll
+    for (int off = 16; off >= kLanes; off >>= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], off);
+    if (g == 0)
+        *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)(first + row) * p.hq + h) * D + 8 * c) =
+            make_uint4(pack_bf16x2(o[0] / l, o[1] / l), pack_bf16x2(o[2] / l, o[3] / l), pack_bf16x2(o[4] / l, o[5] / l), pack_bf16x2(o[6] / l, o[7] / l));
+}
+
+// Rows of 32 that came out non-finite (bits of `rows`; a lane's row is row0 + lane): which of them the tensor cores may have
+// got wrong, and those again.
+//
+// A row whose logits jumped (bits of `jumped`) is one.  Of the others the products are right but for what masked values of
+// the last block add, 0 times an infinity: a column of O that is not finite for another reason has met a value that is not
+// finite in the blocks before, all of whose keys the row sees.  So a column that is finite there and is not in the result sends
+// its row to be computed again, and the rest stays as it is.  That bounds the work: one undefined value early in a
+// sequence makes every later row undefined, but only rows of the blocks in which a column first became so are computed
+// again, at most 128 for each column.
+template <int D>
+__device__ __noinline__ void mend_rows(const PromptParams& p, int first, int row0, int before, int h, unsigned rows, unsigned jumped) {
+    constexpr int kLanes = D / 8, kKeys = 32 / kLanes;
+    const int lane = threadIdx.x & 31, c = lane % kLanes, g = lane / kLanes;
+    uint32_t top[4] = {0u, 0u, 0u, 0u};                        // of the values before: largest magnitudes of the lane's eight columns
+    if ((rows & ~jumped) != 0) {
+        const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v) + (long long)first * p.v_stride + (long long)(h / p.group) * D + 8 * c;
+        for (int key0 = 0; key0 < before; key0 += 64) {        // (before: a multiple of 128)
+#pragma unroll
+            for (int i = 0; i < 64 / kKeys; ++i) {
+                const uint4 x = *reinterpret_cast<const uint4*>(v + (key0 + i * kKeys + g) * p.v_stride);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e] = __vmaxu2(top[e], w[e] & 0x7fff7fffu);
+            }
+        }
+#pragma unroll
+        for (int off = 16; off >= kLanes; off >>= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[e] = __vmaxu2(top[e], __shfl_xor_sync(0xffffffffu, top[e], off));
+    }
+    for (; rows != 0; rows &= rows - 1) {
+        const int i = __ffs(rows) - 1;
+        bool again = (jumped >> i & 1) != 0;
+        if (!again) {
+            const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.out) + ((long long)(first + row0 + i) * p.hq + h) * D + 8 * c);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                again = again || ((w[e] & 0x7f80u) == 0x7f80u && (top[e] & 0xffffu) < 0x7f80u) || ((w[e] & 0x7f800000u) == 0x7f800000u && top[e] < 0x7f800000u);
+        }
+        if (__any_sync(0xffffffffu, again)) prompt_row<D>(p, first, row0 + i, h);
+    }
+    __syncwarp();
 }
 
 // 2^x of two numbers on the multipliers, for x >= -125 (below, and for minus infinity and NaN, 2^-125): 2^n 2^f with n the nearest whole number and 2^f a
@@ -393,6 +480,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         sm.slow = 0;
+        for (int i = 0; i < 8; ++i) sm.jumped[i] = 0u;
         mbar_init(smem_u32(&sm.q_full), 1);
         mbar_init(smem_u32(&sm.q_empty), 1);
         mbar_init(smem_u32(&sm.drained), 1);
@@ -660,7 +748,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     sums[0] = mul_f32x2(sums[0], corr2);
                     sums[1] = mul_f32x2(sums[1], corr2);
                     // a jump that P, up to 2^127 in bf16, or O would not hold: the row is computed again at the end
-                    if (top_x > ref + 100.f) sums[0] = pack_f32x2(__int_as_float(0x7fc00000), 0.f);
+                    const unsigned far = __ballot_sync(0xffffffffu, row < t.y && top_x > ref + 100.f);
+                    if (far != 0) {
+                        if (top_x > ref + 100.f) sums[0] = pack_f32x2(__int_as_float(0x7fc00000), 0.f);
+                        if (lane == 0) sm.jumped[warp] |= far;
+                    }
                     if (grown) ref = top_x;
                 }
                 if (j == n - 1) block(Flag<true>()); else block(Flag<false>());
@@ -669,7 +761,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             unpack_f32x2(add_f32x2(sums[0], sums[1]), sum, sum1);
             sum += sum1;
             // (an undefined or infinite logit makes the row undefined, and so do logits that are minus infinity without exception)
-            if (!(top_x > kPtLowest && top_x <= fminf(ref + 100.f, 3.4028235e38f))) sum = __int_as_float(0x7fc00000);
+            const bool defined = top_x > kPtLowest && top_x <= 3.4028235e38f;
+            if (!(defined && top_x <= ref + 100.f)) sum = __int_as_float(0x7fc00000);
             // the result
             wait_phase(smem_u32(&sm.o_full[h]), o_count & 1, p.status, dead, &sm.slow);
             ++o_count;
@@ -697,12 +790,18 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             tcgen05_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.o_empty[h]));
-            unsigned again = __ballot_sync(0xffffffffu, row < t.y && top >= 0x7f800000u);
-            if (again != 0) {                                  // (row by row: the other warps' waits have to be patient)
-                if (lane == 0) atomicAdd(&sm.slow, 1);
-                for (; again != 0; again &= again - 1) prompt_row<D>(p, t.x, row - lane + __ffs(again) - 1, t.w);
+            if (__any_sync(0xffffffffu, row < t.y && top >= 0x7f800000u)) {      // rows that are not finite
+                const unsigned jumped = (sm.jumped[warp] | __ballot_sync(0xffffffffu, top_x > ref + 100.f)) & __ballot_sync(0xffffffffu, defined);
+                const bool mine = jumped >> lane & 1;
+                // (a row whose sum is undefined without a jump is undefined with cause, in every column)
+                const unsigned rows = __ballot_sync(0xffffffffu, row < t.y && top >= 0x7f800000u && (sum == sum || mine));
                 __syncwarp();
-                if (lane == 0) atomicSub(&sm.slow, 1);
+                if (lane == 0) sm.jumped[warp] = 0u;
+                if (rows != 0) {                               // (row by row: the other warps' waits have to be patient)
+                    if (lane == 0) atomicAdd(&sm.slow, 1);
+                    mend_rows<D>(p, t.x, row - lane, (n - 1) * kPtBlock, t.w, rows, jumped);
+                    if (lane == 0) atomicSub(&sm.slow, 1);
+                }
             }
         }
     }
