@@ -456,8 +456,8 @@ int ts_norm_rotate(const ts_norm_rotate_args* args);
  * Causal attention of whole prompts: `batch` sequences packed one behind the other, sequence b being the tokens
  * cu_seqlens[b] .. cu_seqlens[b+1]-1; token i attends to the tokens of its own sequence up to itself.  q and k come already
  * rotated (ts_norm_rotate).  Query head h reads KV head h / (hq/hkv).  Lengths of zero and one are lengths like any other.
- * cu_seqlens is read on the device; a bound outside [0, tokens] or below the one before it ends the sequence there and is
- * reported (TS_ERR_BAD_LENGTH).  Rows of `out` that belong to no sequence (those behind the last one among them) are left as
+ * cu_seqlens is read on the device; a bound outside [0, tokens] or below one before it ends the sequence there, the next one
+ * starts behind all before it (no token belongs to two), and is reported (TS_ERR_BAD_LENGTH).  Rows of `out` that belong to no sequence (those behind the last one among them) are left as
  * they were.  No value of one sequence reaches another, infinities and NaN included; inside
  * a sequence they reach the tokens that attend to them.
  * In bf16 the softmax weights enter the second product in bf16, all sums are fp32; in fp32 everything is fp32.

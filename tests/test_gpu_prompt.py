@@ -389,3 +389,40 @@ def test_an_early_undefined_value_does_not_hold_the_call_up(columns):
     bad[3:, :, columns] = True
     assert int(status) == 0 and torch.equal(~torch.isfinite(out), bad)
     assert took[1] <= 10 * took[0], took
+
+
+def _in_order(cu, tokens):
+    """Bounds that give the sequences that are left of `cu`: each ends where it still does, behind all before it."""
+    got, high = [], 0
+    for x in cu:
+        high = max(high, min(max(x, 0), tokens))
+        got.append(high)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+def test_sequences_of_bounds_out_of_order_share_no_token(dtype):
+    """A bound below one before it, or outside the tokens, ends its sequence; the next one starts behind all before it, so no token
+    is written twice and none of a sequence's tokens is left out.  Sequences by the dozen, over the edges of what a warp looks
+    at together, among them."""
+    g = torch.Generator().manual_seed(59)
+    q, k, v, _ = _prompt_case(59, 4, 2, 64, [500], dtype)
+    args = [t.cuda() for t in (q, k, v)]
+    cases = [[0, 100, 50, 200], [0, 50, 900], [-5, 50, 500], [30, 20, 60], [0, 90, 10, 80, 200, 150, 300, 299, 500], [500, 0, 500], [100, 0, 100, 0, 500, 0, 500]]
+    cases += [torch.randint(-50, 600, (n,), generator=g).tolist() for n in (33, 34, 70, 300)]
+    ordered = torch.randint(0, 501, (300,), generator=g).sort()[0]
+    for at in (31, 32, 33, 64, 200, 299):
+        case = ordered.clone()
+        case[at] = int(case[at - 1]) - 40
+        cases.append(case.tolist())
+    for case in cases:
+        good = _in_order(case, 500)
+        outs = []
+        for cu in (case, good):
+            status = torch.zeros(1, dtype=torch.int32, device="cuda")
+            out = torch.full_like(args[0], 7.0)
+            prompt.prompt_attend(*args, torch.tensor(cu, dtype=torch.int32, device="cuda"), 0.1, out=out, status=status)
+            assert int(status) == (7 if cu != good else 0), case
+            outs.append(out)
+        assert torch.equal(outs[0], outs[1]), case
+        assert bool((outs[0][:good[0]] == 7.0).all()) and bool((outs[0][good[-1]:] == 7.0).all()) and not bool((outs[0][good[0]:good[-1]] == 7.0).any())

@@ -25,12 +25,36 @@ struct PromptParams {
     int* status;
 };
 
-// Sequence b: first token and length.  Bounds that make no sense are reported and cut.
-__device__ __forceinline__ int2 sequence_of(const PromptParams& p, int b) {
-    const int a = p.cu[b], e = p.cu[b + 1];
-    const int first = min(max(a, 0), p.tokens), end = min(max(e, first), p.tokens);
-    if (a != first || e != end) report(p.status, TS_ERR_BAD_LENGTH);
+// Bounds that make no sense are reported and cut: a sequence lies in [0, tokens) and behind all before it, so no two of them share
+// a token, and there are never more tiles than tokens and sequences allow.
+__device__ __forceinline__ int bound_of(const PromptParams& p, int b) { return min(max(p.cu[b], 0), p.tokens); }
+// Sequence b: first token and length; `floor`: the largest bound before it, and then with its own.
+__device__ __forceinline__ int2 sequence_of(const PromptParams& p, int b, int& floor) {
+    const int first = max(bound_of(p, b), floor), end = max(bound_of(p, b + 1), first);
+    if (p.cu[b] != first || p.cu[b + 1] != end) report(p.status, TS_ERR_BAD_LENGTH);
+    floor = end;
     return make_int2(first, end - first);
+}
+// The same for 32 sequences, a lane each (none behind the last).  All lanes call, for base = 0, 32, ... in turn.
+__device__ __forceinline__ int2 sequences_of(const PromptParams& p, int base, int& floor) {
+    const int lane = threadIdx.x & 31, b = base + lane;
+    const bool in = b < p.batch;
+    int first = in ? bound_of(p, b) : 0, end = in ? bound_of(p, b + 1) : 0;
+    if (__any_sync(0xffffffffu, in && (first < floor || end < first))) {          // out of order
+        int high = max(first, end);                            // of the bounds so far
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, high, off);
+            if (lane >= off) high = max(high, t);
+        }
+        high = max(high, floor);
+        const int before = __shfl_up_sync(0xffffffffu, high, 1);
+        first = max(first, lane == 0 ? floor : before);
+        end = high;
+    }
+    if (in && (p.cu[b] != first || p.cu[b + 1] != end)) report(p.status, TS_ERR_BAD_LENGTH);
+    floor = __shfl_sync(0xffffffffu, end, 31);
+    return make_int2(first, in ? end - first : 0);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -58,16 +82,28 @@ struct PromptPlainSmem {
 template <int D>
 __device__ __forceinline__ bool find_tile(const PromptParams& p, int tile, PromptPlainSmem<D>& sm) {
     const int per = (p.batch + kPpThreads - 1) / kPpThreads, b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += (sequence_of(p, b).y + kPpRows - 1) / kPpRows;
+    bool order = true;
+    for (int b = b0; b < b1; ++b) order = order && p.cu[b] <= p.cu[b + 1];
+    int floor0 = 0;                                            // largest bound before the thread's sequences, if it is above their first
+    if (__syncthreads_or(!order)) {
+        int high = 0;
+        for (int b = b0; b < b1; ++b) high = max(high, max(bound_of(p, b), bound_of(p, b + 1)));
+        sm.tiles[threadIdx.x] = high;
+        __syncthreads();
+        for (int i = 0; i < threadIdx.x; ++i) floor0 = max(floor0, sm.tiles[i]);
+        __syncthreads();
+    }
+    int sum = 0, floor = floor0;
+    for (int b = b0; b < b1; ++b) sum += (sequence_of(p, b, floor).y + kPpRows - 1) / kPpRows;
     sm.tiles[threadIdx.x] = sum;
     if (threadIdx.x == 0) sm.found[1] = 0;
     __syncthreads();
     int before = 0;
     for (int i = 0; i < threadIdx.x; ++i) before += sm.tiles[i];
     if (tile >= before && tile < before + sum) {
+        floor = floor0;
         for (int b = b0; b < b1; ++b) {
-            const int2 s = sequence_of(p, b);
+            const int2 s = sequence_of(p, b, floor);
             const int n = (s.y + kPpRows - 1) / kPpRows;
             if (tile < before + n) {
                 sm.found[0] = s.x; sm.found[1] = s.y; sm.found[2] = n - 1 - (tile - before);
@@ -296,24 +332,26 @@ __device__ __forceinline__ int blocks_of(int len, int tile, int h) {
 struct TileOrder {
     int level, from;                                           // tiles of this number start at position `from`
 };
-__device__ __forceinline__ int tiles_of(const PromptParams& p, int b) { return b < p.batch ? (sequence_of(p, b).y + 2 * kPtRows - 1) / (2 * kPtRows) : 0; }
+__device__ __forceinline__ int tiles_of(int2 sequence) { return (sequence.y + 2 * kPtRows - 1) / (2 * kPtRows); }
 __device__ int count_tiles(const PromptParams& p, int above) {     // sequences with more tiles than `above`; all lanes call
-    int n = 0;
-    for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += tiles_of(p, b) > above;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+    int n = 0, floor = 0;
+    for (int base = 0; base < p.batch; base += 32) n += __popc(__ballot_sync(0xffffffffu, tiles_of(sequences_of(p, base, floor)) > above));
     return n;
 }
-// Sequence at place `rank` among those with more tiles than `level`.
-__device__ int sequence_at(const PromptParams& p, int level, int rank) {
-    const int lane = threadIdx.x & 31;
+// The sequence (first token, length) at place `rank` among those with more tiles than `level`; all lanes call.
+__device__ int2 sequence_at(const PromptParams& p, int level, int rank) {
+    int floor = 0;
     for (int base = 0; base < p.batch; base += 32) {
-        const unsigned has = __ballot_sync(0xffffffffu, tiles_of(p, base + lane) > level);
+        const int2 s = sequences_of(p, base, floor);
+        const unsigned has = __ballot_sync(0xffffffffu, tiles_of(s) > level);
         const int n = __popc(has);
-        if (rank < n) return base + __fns(has, 0, rank + 1);
+        if (rank < n) {
+            const int from = __fns(has, 0, rank + 1);
+            return make_int2(__shfl_sync(0xffffffffu, s.x, from), __shfl_sync(0xffffffffu, s.y, from));
+        }
         rank -= n;
     }
-    return 0;
+    return make_int2(0, 0);
 }
 
 // Row `row` of a sequence for one head on the CUDA cores, by one warp: D/8 lanes hold a key's or a value's row, eight elements each,
@@ -522,8 +560,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         // ---------------- requests ----------------
         TileOrder order = {0, 0};
         {
-            int most = 0;
-            for (int b = lane; b < p.batch; b += 32) most = max(most, tiles_of(p, b));
+            int most = 0, floor = 0;
+            for (int base = 0; base < p.batch; base += 32) most = max(most, tiles_of(sequences_of(p, base, floor)));
 #pragma unroll
             for (int off = 16; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
             order.level = most - 1;
@@ -541,7 +579,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             }
             int4 t = make_int4(0, -1, 0, head);
             if (order.level >= 0 && !dead) {
-                const int2 seq = sequence_of(p, sequence_at(p, order.level, pos - order.from));
+                const int2 seq = sequence_at(p, order.level, pos - order.from);
                 t = make_int4(seq.x, seq.y, order.level, head);
             }
             const int i = put % kPtQueue;
