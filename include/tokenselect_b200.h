@@ -370,10 +370,12 @@ typedef struct ts_quant_rows_args {
 } ts_quant_rows_args;
 
 /* Quantise `count` rows into the pool.  A row outside [0, pool_rows) is skipped and reported (TS_ERR_BAD_SLOT).  A pool row
- * that is listed twice in one call is left with a mixture of the rows given for it. */
+ * that is listed twice in one call is left with a mixture of the rows given for it.  k, v and rows share no byte with the pool
+ * (TS_ERR_INVALID_ARG). */
 int ts_quant_write(const ts_quant_rows_args* args);
 
-/* Read `count` rows back.  A row outside [0, pool_rows) gives zeros and is reported (TS_ERR_BAD_SLOT). */
+/* Read `count` rows back.  A row outside [0, pool_rows) gives zeros and is reported (TS_ERR_BAD_SLOT).  k, v, rows and the pool share
+ * no byte (TS_ERR_INVALID_ARG); slices of one buffer with gaps for each other do not. */
 int ts_quant_read(const ts_quant_rows_args* args);
 
 /*
@@ -386,7 +388,7 @@ int ts_quant_read(const ts_quant_rows_args* args);
  * In bf16 the rotated keys and queries and the softmax weights enter the products in fp16 (the queries scaled by a power of
  * two into its range), all sums are fp32; in fp32 everything is fp32.
  * `workspace` holds the partial results of one call (ts_quant_attend_workspace() bytes, any contents): calls that may run
- * at the same time need one each.
+ * at the same time need one each.  It shares no byte with the call's tensors, nor `out` with any but q (TS_ERR_INVALID_ARG).
  */
 typedef struct ts_quant_attend_args {
     uint32_t struct_size;          /* sizeof(ts_quant_attend_args), checked */
@@ -425,7 +427,8 @@ int ts_quant_attend(const ts_quant_attend_args* args);
  *   y = x * rsqrt(mean(x^2) + eps) * weight        (no norm where the weight is NULL)
  *   (y_i, y_{i+head_dim/2}) turned by position * rope_base^(-2i/head_dim) / rope_scale    (no rotation where positions is NULL)
  * in fp32, rounded once.  k_plain, if not NULL, takes the normed keys before the rotation: what a cache of un-rotated keys
- * keeps.  Outputs are contiguous [tokens, heads, head_dim]; an output may be the (contiguous) input of the same name.
+ * keeps.  Outputs are contiguous [tokens, heads, head_dim]; an output may be the whole place of the (contiguous) input that it is
+ * made of, and shares no byte with another tensor of the call otherwise (TS_ERR_INVALID_ARG).
  */
 typedef struct ts_norm_rotate_args {
     uint32_t struct_size;          /* sizeof(ts_norm_rotate_args), checked */

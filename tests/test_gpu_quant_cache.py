@@ -371,3 +371,21 @@ def test_far_positions_turn_by_exact_angles(dtype):
                         torch.tensor([n], dtype=torch.int32, device="cuda"), scale, 1e4)
     err = (out.cpu().double().view_as(want) - want).abs()
     assert bool((err <= tol + 1e-12).all()), float((err / mag).max())
+
+
+def test_a_workspace_apart_from_the_tensors():
+    """A workspace that shares memory with the call's tensors is refused before a launch; the output may take the query's place."""
+    import tokenselect_b200
+    hq, hkv, d = 8, 2, 128
+    q, pool, rtt, slots, lens = (t.cuda() for t in _attend_case(73, hq, hkv, d, [50, 300], BF16))
+    need = qc.kv4_attend_workspace(2, hq, d)
+    want = qc.kv4_attend(q, pool, rtt, slots, lens, 0.1, 5e5)
+    both = torch.zeros(need + q.numel() * 2, dtype=torch.uint8, device="cuda")
+    for at in (0, need - 64):
+        inside = both[at:at + q.numel() * 2].view(BF16).view(q.shape)
+        inside.copy_(q)
+        for kw in ({"out": inside}, {}):
+            with pytest.raises(tokenselect_b200.TokenSelectError):
+                qc.kv4_attend(q if kw else inside, pool, rtt, slots, lens, 0.1, 5e5, workspace=both[:need], **kw)
+    own = q.clone()
+    assert qc.kv4_attend(own, pool, rtt, slots, lens, 0.1, 5e5, out=own, workspace=both[:need]) is own and torch.equal(own, want)

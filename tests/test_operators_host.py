@@ -149,3 +149,96 @@ def test_plain_attention_skips_what_is_not_seen():
     o, mag = ref.attend(q, k, v, seen, 0.1)
     assert torch.allclose(o[0, 0], v[0, 0].double()) and torch.isfinite(o).all() and not o[2].any() and (mag >= o.abs() - 1e-12).all()
     assert torch.equal(ref.causal([1, 0, 2], 3), torch.tensor([[1, 0, 0], [0, 1, 0], [0, 1, 1]], dtype=torch.bool))
+
+
+def test_extents_meet_where_their_bytes_do(tmp_path):
+    """The host's rule for what two tensors of a call share, against sets of bytes."""
+    (tmp_path / "x.cpp").write_text("""
+        #include "extent.h"
+        #include <set>
+        #include <random>
+        #include <cstdio>
+        using namespace ts;
+        static std::set<uintptr_t> bytes(uintptr_t p, uint64_t b, uint64_t s, uint64_t n) {
+            std::set<uintptr_t> r;
+            for (uint64_t i = 0; i < n; ++i) for (uint64_t j = 0; j < b; ++j) r.insert(p + i * s + j);
+            return r;
+        }
+        int main() {
+            std::mt19937 g(1);
+            auto in = [&](int lo, int hi) { return lo + (int)(g() % (hi - lo + 1)); };
+            int met = 0;
+            for (int k = 0; k < 200000; ++k) {
+                uint64_t b[2], s[2], n[2]; uintptr_t p[2];
+                for (int i = 0; i < 2; ++i) { b[i] = in(0, 6); n[i] = in(0, 5); s[i] = b[i] + (in(0, 2) ? in(0, 12) : 0); p[i] = in(1, 60); }
+                if (in(0, 1)) s[1] = s[0] < b[1] ? b[1] : s[0];
+                auto x = bytes(p[0], b[0], s[0], n[0]), y = bytes(p[1], b[1], s[1], n[1]);
+                bool want = false;
+                for (auto v : x) want = want || y.count(v);
+                met += want;
+                if (overlap(Extent((void*)p[0], b[0], s[0], n[0]), Extent((void*)p[1], b[1], s[1], n[1])) != want) {
+                    printf("%d: %d %d %d %d, %d %d %d %d\\n", k, (int)p[0], (int)b[0], (int)s[0], (int)n[0], (int)p[1], (int)b[1], (int)s[1], (int)n[1]);
+                    return 1;
+                }
+            }
+            return met > 20000 && met < 180000 ? 0 : 2;
+        }""")
+    subprocess.check_call(["g++", "-std=c++17", "-I", build.CSRC, str(tmp_path / "x.cpp"), "-o", str(tmp_path / "x")])
+    subprocess.check_call([str(tmp_path / "x")])
+
+
+NOWHERE = 1 << 20                # no such device: what is not refused before ends there (3), and nothing is launched
+
+
+def _far(**kw):
+    """Pointers far apart from each other."""
+    return {name: (i + 1) << 32 for i, name in enumerate(kw.pop("names").split())} | kw
+
+
+def test_calls_refuse_outputs_that_share_memory(lib):
+    def norm(**kw):
+        return lib.ts_norm_rotate(C.byref(_norm(device=NOWHERE, **(_far(names="q k positions q_weight k_weight q_out k_out k_plain") | kw))))
+    p = _far(names="q k positions q_weight k_weight q_out k_out k_plain")
+    row = 4 * 128 * 2                                                         # bytes of a token's queries; of its keys half
+    assert norm() == 3
+    assert norm(q_out=p["q"]) == norm(k_out=p["k"]) == norm(k_plain=p["k"]) == norm(q_out=p["q"], k_out=p["k"]) == 3          # in place
+    for shift in (2, row, 2 * row, -2, -2 * row):
+        assert norm(q_out=p["q"] + shift) == 1
+    assert norm(q_out=p["q"] + 3 * row) == norm(q_out=p["q"] - 3 * row) == 3
+    assert norm(q_out=p["q"], q_stride=1024) == norm(q_out=p["q"] + row, q_stride=1024) == 1 and norm(q_out=p["q"], q_stride=1024, tokens=1) == 3
+    assert norm(q_out=p["q"] + row, q_stride=5 * 512) == 3 and norm(q_out=p["q"] + row, q_stride=4 * 512 - 8) == 1            # the gap behind a token
+    for bad in (dict(q_out=p["k"]), dict(k_out=p["q"] + 8), dict(k_plain=p["q"] + row), dict(k_plain=p["k"] + 256), dict(k_out=p["k"] + 256),
+                dict(q_out=p["k_out"] - row), dict(k_plain=p["k_out"]), dict(k_plain=p["q_out"] + 8), dict(k_out=p["positions"]), dict(q_out=p["k_weight"] - 8)):
+        assert norm(**bad) == 1, bad
+
+    names = "q k v cu_seqlens out"
+    p = _far(names=names)
+
+    def call(**kw):
+        return lib.ts_prompt_attend(C.byref(_prompt(device=NOWHERE, **(p | kw))))
+    assert call() == 3 and call(k=p["q"], v=p["q"]) == 3
+    out = 10 * row
+    for x, stride in (("q", 512), ("k", 256), ("v", 1024)):
+        end = ((9 * stride) + (512 if x == "q" else 256)) * 2
+        assert call(out=p[x]) == call(out=p[x] + 16) == call(out=p[x] + end - 16) == call(out=p[x] - out + 16) == 1
+        assert call(out=p[x] + end) == call(out=p[x] - out) == 3
+    assert call(out=p["cu_seqlens"] - 16) == 1 and call(out=p["cu_seqlens"] + 16) == 3
+
+    p = _far(names="k v rows pool")
+
+    def rows(call, **kw):
+        return call(C.byref(_rows(device=NOWHERE, **(p | kw))))
+    half, pool = 1024 * 2, 10 * 8 * 144
+    for c in (lib.ts_quant_write, lib.ts_quant_read):
+        assert rows(c) == 3
+        assert rows(c, k=p["v"] + half, k_stride=2048, v_stride=2048) == 3                               # K behind V in one buffer
+        assert rows(c, k=p["pool"] + pool - 16) == rows(c, v=p["pool"] - 16) == rows(c, rows=p["pool"] + 4) == 1
+        assert rows(c, k=p["pool"] + pool) == rows(c, v=p["pool"] - 4 * half) == 3
+    assert rows(lib.ts_quant_write, k=p["v"]) == 3                                                       # reading the same rows twice is no harm
+    assert rows(lib.ts_quant_read, k=p["v"]) == rows(lib.ts_quant_read, k=p["v"] + 2 * half) == rows(lib.ts_quant_read, k=p["v"] + half, k_stride=2047, v_stride=2048) == 1
+    assert rows(lib.ts_quant_read, v=p["rows"] - 8) == 1
+
+    p = _far(names="q pool req_to_token req_pool_indices seq_lens out workspace")
+    for bad in ("pool", "req_to_token", "req_pool_indices", "seq_lens"):
+        assert lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **(p | {"out": p[bad] + 4})))) == 1, bad
+    assert lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **p))) == 3 == lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **(p | {"out": p["q"]}))))

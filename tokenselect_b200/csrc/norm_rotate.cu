@@ -188,6 +188,20 @@ extern "C" int ts_norm_rotate(const ts_norm_rotate_args* a) {
     if (a->positions && (!(a->rope_base > 0.0) || !(a->rope_scale > 0.0))) return TS_ERR_INVALID_ARG;
     if (a->tokens == 0) return TS_OK;
     if (!a->q || !a->k || !a->q_out || !a->k_out) return TS_ERR_INVALID_ARG;
+    {
+        // A token's rows are read by others than those that write them, so an output is an input's whole place or no part of it.
+        const uint64_t es = a->dtype == TS_DTYPE_BF16 ? 2 : 4, n = (uint64_t)a->tokens, qb = (uint64_t)a->hq * a->head_dim * es, kb = (uint64_t)a->hkv * a->head_dim * es;
+        const Extent q(a->q, qb, a->q_stride * es, n), k(a->k, kb, a->k_stride * es, n);
+        const Extent small[3] = {{a->positions, 4 * n}, {a->q_weight, a->head_dim * es}, {a->k_weight, a->head_dim * es}};
+        const Extent outs[3] = {{a->q_out, qb * n}, {a->k_out, kb * n}, {a->k_plain, kb * n}};
+        for (int i = 0; i < 3; ++i) {
+            const Extent &own = i == 0 ? q : k, &other = i == 0 ? k : q;
+            const bool in_place = outs[i].at == own.at && own.n == 1;
+            if ((!in_place && overlap(outs[i], own)) || overlap(outs[i], other) || overlap(outs[i], outs[(i + 1) % 3])) return TS_ERR_INVALID_ARG;
+            for (const Extent& s : small)
+                if (overlap(outs[i], s)) return TS_ERR_INVALID_ARG;
+        }
+    }
     const DeviceScope scope(a->device);
     if (!scope.ok) return TS_ERR_CUDA;
     NormParams p;

@@ -903,6 +903,13 @@ extern "C" int ts_prompt_attend(const ts_prompt_args* a) {
     const uintptr_t bits = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v) |
                            reinterpret_cast<uintptr_t>(a->out) | (uintptr_t)((a->q_stride | a->k_stride | a->v_stride) * es);
     if (bits % 16 != 0) return TS_ERR_INVALID_ARG;
+    {
+        const uint64_t n = (uint64_t)a->tokens, qb = (uint64_t)a->hq * a->head_dim * es, kb = (uint64_t)a->hkv * a->head_dim * es;
+        const Extent out(a->out, qb * n);
+        if (overlap(out, Extent(a->q, qb, a->q_stride * es, n)) || overlap(out, Extent(a->k, kb, a->k_stride * es, n)) ||
+            overlap(out, Extent(a->v, kb, a->v_stride * es, n)) || overlap(out, Extent(a->cu_seqlens, 4 * ((uint64_t)a->batch + 1))))
+            return TS_ERR_INVALID_ARG;
+    }
     const DeviceScope scope(a->device);
     if (!scope.ok) return TS_ERR_CUDA;
     PromptParams p;

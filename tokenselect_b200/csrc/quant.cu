@@ -187,6 +187,13 @@ int quant_rows(const ts_quant_rows_args* a, bool write) {
     if (!power_of_two(a->k_scale) || !power_of_two(a->v_scale)) return TS_ERR_INVALID_ARG;
     if (a->count == 0) return TS_OK;
     if (!a->k || !a->v || !a->rows || !a->pool || reinterpret_cast<uintptr_t>(a->pool) % 16 != 0) return TS_ERR_INVALID_ARG;
+    {
+        const uint64_t es = a->dtype == TS_DTYPE_BF16 ? 2 : 4, n = (uint64_t)a->count, row = (uint64_t)a->hkv * a->head_dim * es;
+        const Extent k(a->k, row, a->k_stride * es, n), v(a->v, row, a->v_stride * es, n), rows(a->rows, 4 * n);
+        const Extent pool(a->pool, (uint64_t)a->pool_rows * a->hkv * (a->head_dim * 9 / 8));
+        if (overlap(k, pool) || overlap(v, pool) || overlap(rows, pool)) return TS_ERR_INVALID_ARG;
+        if (!write && (overlap(k, v) || overlap(k, rows) || overlap(v, rows))) return TS_ERR_INVALID_ARG;
+    }
     const DeviceScope scope(a->device);
     if (!scope.ok) return TS_ERR_CUDA;
     QuantRowsParams p;

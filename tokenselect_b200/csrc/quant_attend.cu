@@ -929,10 +929,18 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     if (a->batch == 0) return TS_OK;
     if (!a->q || !a->pool || !a->req_to_token || !a->req_pool_indices || !a->seq_lens || !a->out || !a->workspace) return TS_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(a->pool) % 16 != 0 || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return TS_ERR_INVALID_ARG;
+    // (`out` may be `q`: it is written when all queries have been read.)
+    const uint64_t heads = (uint64_t)a->batch * a->hq * a->head_dim * (a->dtype == TS_DTYPE_BF16 ? 2 : 4);
+    const Extent out(a->out, heads), q(a->q, heads), pool(a->pool, (uint64_t)a->pool_rows * a->hkv * (a->head_dim * 9 / 8));
+    const Extent table(a->req_to_token, 4 * (uint64_t)a->max_ctx, 4 * (uint64_t)a->req_to_token_stride, a->max_reqs);
+    const Extent slots(a->req_pool_indices, 4 * (uint64_t)a->batch), lens(a->seq_lens, 4 * (uint64_t)a->batch);
+    if (overlap(out, pool) || overlap(out, table) || overlap(out, slots) || overlap(out, lens)) return TS_ERR_INVALID_ARG;
     const int sms = sms_of(a->device);
     if (sms <= 0) return TS_ERR_CUDA;
     const int pieces = attend_pieces(a->dtype, a->hkv, sms);
     if (a->workspace_bytes < partial_bytes(sms, a->batch, a->hq, a->head_dim)) return TS_ERR_CAPACITY;
+    const Extent work(a->workspace, partial_bytes(sms, a->batch, a->hq, a->head_dim));
+    if (overlap(work, out) || overlap(work, q) || overlap(work, pool) || overlap(work, table) || overlap(work, slots) || overlap(work, lens)) return TS_ERR_INVALID_ARG;
     const DeviceScope scope(a->device);
     if (!scope.ok) return TS_ERR_CUDA;
     QuantAttendParams p;

@@ -2,6 +2,7 @@
 #pragma once
 #include <math.h>
 
+#include "extent.h"
 #include "ptx.cuh"
 
 namespace ts {

@@ -51,7 +51,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: Optional[torch.Tens
     (-2 i / head_dim) / rope_scale`` (``positions`` int32 ``[tokens]``; None: no rotation), in one pass, in fp32,
     rounded once.  Returns ``(q, k)``, and behind them the normed keys before the rotation, for the cache, when
     ``with_plain_k`` or ``k_plain`` asks for them.  Inputs may be slices of a fused projection's output; outputs are
-    contiguous, and may be the inputs themselves where those are."""
+    contiguous, and may be the input that they are made of where that is; otherwise they share no memory with the call's
+    other tensors."""
     # One token costs the device less than a generous host path costs Python: one look at each property.
     dev, dtype, shape = q.get_device(), q.dtype, q.shape
     if len(shape) != 3:
@@ -92,7 +93,7 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens:
     """Causal attention of packed prompts: ``q [tokens, heads, head_dim]``, ``k, v [tokens, kv_heads, head_dim]``, q and
     k rotated; sequence ``b`` is the tokens ``cu_seqlens[b] .. cu_seqlens[b+1] - 1`` (int32 ``[sequences + 1]`` on the
     device, lengths of zero allowed).  Query head ``h`` reads KV head ``h // group``.  Returns ``[tokens, heads,
-    head_dim]``; rows behind the last sequence are left as they were in ``out``.  The tensors start on 16 bytes and
+    head_dim]`` (``out`` shares no memory with the inputs); rows behind the last sequence are left as they were in ``out``.  The tensors start on 16 bytes and
     their tokens lie a multiple of 16 bytes apart (slices of a fused projection do).  ``status`` (optional, int32) is
     set when a bound of ``cu_seqlens`` makes no sense; the sequence then ends where it still does, and the next one starts
     behind all before it."""

@@ -97,7 +97,7 @@ def kv4_read(pool: torch.Tensor, rows: torch.Tensor, dtype: torch.dtype = torch.
              v_scale: float = 1.0, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None,
              status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(k, v) [n, num_kv_heads, head_dim]`` of the pool rows ``rows [n]``: the values their codes stand for, exact in
-    bf16 and in fp32.  ``k`` and ``v`` may be given (rows of a bf16 pool's slice, say).  A row outside the pool gives
+    bf16 and in fp32.  ``k`` and ``v`` may be given (rows of a bf16 pool's slice, say), apart from each other and from the pool.  A row outside the pool gives
     zeros and is reported."""
     d = _check_pool(pool)
     shape = (rows.numel(), pool.shape[1], d)
@@ -132,7 +132,8 @@ def kv4_attend(q: torch.Tensor, pool: torch.Tensor, req_to_token: torch.Tensor, 
     ``decode_layer``.  A request of length 0 (a padded slot of a captured batch) gets zeros.
 
     ``workspace``: uint8, at least :func:`kv4_attend_workspace` bytes, for callers that must not allocate; calls that
-    may run at the same time need one each.  By default every call takes its own from PyTorch's allocator."""
+    may run at the same time need one each.  By default every call takes its own from PyTorch's allocator.
+    ``out`` may be ``q``."""
     d, dev, (pool_rows, hkv, _) = _check_pool(pool), pool.get_device(), pool.shape
     i32, dtype, batch, total = torch.int32, q.dtype, q.shape[0], q.numel()
     if out is None:
