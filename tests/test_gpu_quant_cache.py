@@ -389,3 +389,16 @@ def test_a_workspace_apart_from_the_tensors():
                 qc.kv4_attend(q if kw else inside, pool, rtt, slots, lens, 0.1, 5e5, workspace=both[:need], **kw)
     own = q.clone()
     assert qc.kv4_attend(own, pool, rtt, slots, lens, 0.1, 5e5, out=own, workspace=both[:need]) is own and torch.equal(own, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_queries_of_zeros_and_the_smallest_pool_scale(cap, dtype):
+    """A head of zeros attends to every row alike, whatever the pool's scale of K: the mean of its values.  So does one whose
+    logits are too small for fp32."""
+    hq, hkv, d = 8, 2, 128
+    case = list(_attend_case(67, hq, hkv, d, [17, 40, 160], dtype))
+    case[0].view(3, hq, d)[:, ::2] = 0.0
+    case[0].view(3, hq, d)[:, 1] = 1e-36
+    for gk in (2.0 ** -32, 2.0 ** -21, 1.0):
+        _check_attend(case, hq, d ** -0.5, 5e5, cap=cap, gk=gk)

@@ -544,7 +544,8 @@ __global__ void __launch_bounds__(QtLaunch<PIECE>::kThreads, 1) quant_attend_tc_
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const uint32_t ex = min(max(top >> 7, 1u), 253u);             // biased exponent of the largest element
                 const float down = __uint_as_float((254u - ex) << 23);
-                unit_scale = __uint_as_float(ex << 23) * p.sm_scale;
+                // (never 0, which a masked row's minus infinity is multiplied by: smaller logits than these are all alike)
+                unit_scale = fmaxf(__uint_as_float(ex << 23) * p.sm_scale, 1.17549435e-38f);
 #pragma unroll
                 for (int i = 0; i < 4 * NW; ++i) {
                     x[i] = pack_bf16x2(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down);
