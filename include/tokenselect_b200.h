@@ -341,9 +341,11 @@ int ts_attend_rows_static(const ts_attend_static_args* args);
  * 3, 4, 6 and their negatives), element 2i in the lower half of byte i; sixteen consecutive elements share one 8-bit
  * scale (E4M3).  With the pool's scale g (k_scale or v_scale, a power of two, the same in every call on a pool):
  *   scale = E4M3(min(max|x| / (6 g), 448)), code = E2M1(x / (g * scale)), value = code * scale * g
- * both rounded to nearest, ties to the even code; the codes of a block whose scale rounds to 0 are 0.  A block with an
- * infinity or a NaN reads back as NaN.  Every value is exact in bf16 and in fp32 (while g keeps it in their normal range),
- * so a row read back and written again keeps its codes.  Keys are kept un-rotated, as in the bf16 pools.
+ * both rounded to nearest, ties to the even code; a code has its element's sign, zeros included (8 is minus zero); the codes of a
+ * block whose scale rounds to 0 (largest magnitude 3/512 g or less) are 0.  A block with an infinity or a NaN reads back as NaN.
+ * Every value is exact in bf16 and in fp32 (while g keeps it in their normal range), so a block read back and written again
+ * keeps its bytes if its largest magnitude was above 10/512 g; below, the scale has so few bits that the stored maximum may
+ * choose another.  Keys are kept un-rotated, as in the bf16 pools.
  *
  * These calls take no handle and keep nothing between calls: any number of them may run at the same time, on any
  * streams and in any captured graphs, as long as the caller orders writes and reads of the same rows.

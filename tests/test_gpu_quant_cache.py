@@ -402,3 +402,44 @@ def test_queries_of_zeros_and_the_smallest_pool_scale(cap, dtype):
     case[0].view(3, hq, d)[:, 1] = 1e-36
     for gk in (2.0 ** -32, 2.0 ** -21, 1.0):
         _check_attend(case, hq, d ** -0.5, 5e5, cap=cap, gk=gk)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("g", [1.0, 2.0 ** -20, 2.0 ** 20])
+def test_bytes_written_and_written_again(g, dtype):
+    """The bytes of a pool row are those of the plain quantiser, the sign of an element that rounds to zero among them (a zero
+    keeps its sign too).  Read back and written again, a block whose largest magnitude is above 10/512 of the pool's scale
+    keeps its bytes; of a smaller one the values read back are written like any others."""
+    gen = torch.Generator().manual_seed(3)
+    n, heads, d = 96, 2, 128
+    size = torch.logspace(-2.6, 3.3, n * heads * (d // 16)).view(n, heads, d // 16, 1)       # of a block: scales from 0 to the largest
+    x = (torch.randn(n, heads, d // 16, 16, generator=gen) * size).flatten(-2)
+    x[0, 0, :16] = torch.tensor([3.2, -1.0] + [0.0] * 14) * 2.0 ** -9
+    x[1, 0, :16] = torch.tensor([9.5, -4.0, 0.1, -0.1] + [0.0] * 12) * 2.0 ** -9
+    x[2, 0, :16] = torch.tensor([10.0, -10.0, 0.1, -0.1] + [0.0] * 12) * 2.0 ** -9
+    x[3, 0, :16] = torch.tensor([1e32, -1e3] + [0.0] * 14)
+    x = (x * g).to(dtype)
+    y = x.flip(0).contiguous()
+    rows = torch.arange(n, dtype=torch.int32, device="cuda")
+
+    def written(k, v):
+        pool = qc.kv4_pool(n, heads, d)
+        qc.kv4_write(pool, k.cuda(), v.cuda(), rows, g, g)
+        return pool
+
+    pool = written(x, y)
+    assert torch.equal(pool.cpu(), ref.pack(x, y, g, g))
+    for out in (BF16, F32):
+        k, v = qc.kv4_read(pool, rows, out, g, g)
+        again = written(k, v).cpu()
+        assert torch.equal(torch.stack(ref.unpack(again, g, g)), torch.stack((ref.held(k.cpu(), g), ref.held(v.cpu(), g))))
+        kept = x.double().unflatten(-1, (-1, 16)).abs().amax(-1) > 10.0 / 512.0 * g              # [n, heads, blocks]
+        code = lambda p: p[..., :d // 2].unflatten(-1, (-1, 8))                                  # noqa: E731
+        scale = slice(d, d + d // 16)
+        assert torch.equal(code(again)[kept], code(pool.cpu())[kept]) and torch.equal(again[..., scale][kept], pool.cpu()[..., scale][kept])
+    zero = torch.zeros(n, heads, d)
+    zero[:, :, 0], zero[:, :, 1::2] = 1.0, -0.0
+    for top in (1.0, 2e31):                                                   # beyond 1e30 the quotients are taken another way
+        zero[:, :, ::16] = top
+        z = (zero * g).to(dtype)
+        assert bool((written(z, z)[..., :d // 2] & 0xF0 == 0x80).all()), top

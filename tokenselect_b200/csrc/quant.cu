@@ -72,12 +72,13 @@ __device__ __forceinline__ uint32_t quantise_block(const T (&x)[kQuantBlock], fl
     float y[2][8];
     if (most < 1e30f) {
         // Sixteen quotients by one divisor: Markstein's correction (1990) of the product with the rounded reciprocal gives the
-        // rounded quotient in three operations.
+        // rounded quotient in three operations.  (With the remainder's sign the other way round a zero keeps its own: -0 would
+        // become +0, and a row read back and written again change.)
         const float inv_s = __fdiv_rn(1.f, s);
 #pragma unroll
         for (int e = 0; e < kQuantBlock; ++e) {
             const float v = to_f32<T>(x[e]), q = v * inv_s;
-            y[e >> 3][e & 7] = fmaf(fmaf(-q, s, v), inv_s, q);
+            y[e >> 3][e & 7] = fmaf(-fmaf(q, s, -v), inv_s, q);
         }
     } else {                                                   // far beyond what the scale can hold: the quotient may be infinite
 #pragma unroll

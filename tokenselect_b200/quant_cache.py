@@ -5,9 +5,10 @@ bf16 takes 512): 4-bit floats (E2M1) with one 8-bit scale (E4M3) per sixteen ele
 states the layout and the rounding.  Keys are kept un-rotated, and page size is 1, as in the bf16 pools: the same
 ``req_to_token`` tables, and the row lists that a selection leaves, index them.
 
-``k_scale`` and ``v_scale`` are the pool's scales, powers of two, the same in every call on a pool: values between
-``2**-10 * scale`` and ``2688 * scale`` are held (those of a block together: an element a 24th of its block's
-largest rounds to zero).
+``k_scale`` and ``v_scale`` are the pool's scales, powers of two, the same in every call on a pool: blocks whose largest
+magnitude lies between ``0.006 * scale`` and ``2688 * scale`` are held (an element a 24th of its block's largest
+rounds to zero; a smaller block becomes zeros, a larger one is clamped).  What is read back and written again keeps its
+bytes where a block's largest magnitude was above ``0.02 * scale``.
 
 The functions keep nothing between calls and enqueue on the current stream; they may be captured into CUDA graphs.
 ``status`` (optional, a CUDA int32 tensor) is set to a ``TS_ERR_*`` code when a kernel finds a row outside the pool or
