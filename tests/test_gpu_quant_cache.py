@@ -443,3 +443,15 @@ def test_bytes_written_and_written_again(g, dtype):
         zero[:, :, ::16] = top
         z = (zero * g).to(dtype)
         assert bool((written(z, z)[..., :d // 2] & 0xF0 == 0x80).all()), top
+
+
+def test_type_of_what_is_read():
+    """bf16 by default, what is asked for otherwise, and the given tensors' own; a type that contradicts them is refused."""
+    pool, rows = qc.kv4_pool(4, 2, 64), torch.arange(3, dtype=torch.int32, device="cuda")
+    given = torch.empty(3, 2, 64, dtype=F32, device="cuda")
+    assert [t.dtype for t in qc.kv4_read(pool, rows)] == [BF16, BF16] and [t.dtype for t in qc.kv4_read(pool, rows, F32)] == [F32, F32]
+    for kw in ({"k": given}, {"v": given}, {"k": given, "dtype": F32}):
+        assert [t.dtype for t in qc.kv4_read(pool, rows, **kw)] == [F32, F32]
+    for kw in ({"k": given}, {"v": given}):
+        with pytest.raises(ValueError, match="dtype"):
+            qc.kv4_read(pool, rows, BF16, **kw)

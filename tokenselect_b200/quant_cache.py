@@ -94,16 +94,20 @@ def kv4_write(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: torch.
     check(_lib_().ts_quant_write(C.byref(a)), "ts_quant_write")
 
 
-def kv4_read(pool: torch.Tensor, rows: torch.Tensor, dtype: torch.dtype = torch.bfloat16, k_scale: float = 1.0,
+def kv4_read(pool: torch.Tensor, rows: torch.Tensor, dtype: Optional[torch.dtype] = None, k_scale: float = 1.0,
              v_scale: float = 1.0, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None,
              status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(k, v) [n, num_kv_heads, head_dim]`` of the pool rows ``rows [n]``: the values their codes stand for, exact in
-    bf16 and in fp32.  ``k`` and ``v`` may be given (rows of a bf16 pool's slice, say), apart from each other and from the pool.  A row outside the pool gives
-    zeros and is reported."""
+    bf16 and in fp32 (``dtype``; bf16 by default).  ``k`` and ``v`` may be given (rows of a bf16 pool's slice, say), apart
+    from each other and from the pool; the results then have their type.  A row outside the pool gives zeros and is
+    reported."""
     d = _check_pool(pool)
+    for t in (k, v):
+        if t is not None and dtype is not None and t.dtype != dtype:
+            raise ValueError("dtype must be that of the given k and v")
     shape = (rows.numel(), pool.shape[1], d)
     if k is None:
-        k = pool.new_empty(shape, dtype=dtype if v is None else v.dtype)
+        k = pool.new_empty(shape, dtype=dtype or torch.bfloat16 if v is None else v.dtype)
     if v is None:
         v = torch.empty_like(k, memory_format=torch.contiguous_format)
     a = _row_args(pool, d, k, v, rows, k_scale, v_scale, status)
