@@ -410,9 +410,9 @@ typedef struct ts_quant_attend_args {
     const int32_t* req_pool_indices; /* [batch] */
     const int32_t* seq_lens;       /* [batch] */
     void* out;                     /* [batch, hq*head_dim] */
-    float sm_scale;                /* > 0 */
-    float logit_cap;               /* soft cap, used when > 0 */
-    double rope_base;
+    float sm_scale;                /* > 0, finite */
+    float logit_cap;               /* soft cap, used when > 0; finite */
+    double rope_base;              /* > 0, finite, as rope_scale */
     double rope_scale;
     float k_scale, v_scale;        /* powers of two, 2^-32 .. 2^32 */
     void* workspace;               /* start on a multiple of 16 */
@@ -447,7 +447,7 @@ typedef struct ts_norm_rotate_args {
     const int32_t* positions;      /* [tokens] or NULL */
     const void* q_weight;          /* [head_dim] or NULL */
     const void* k_weight;          /* [head_dim] or NULL */
-    double rope_base;
+    double rope_base;              /* > 0, finite, as rope_scale; not looked at without positions */
     double rope_scale;
     void* q_out;
     void* k_out;
@@ -477,8 +477,8 @@ typedef struct ts_prompt_args {
     int32_t batch;                 /* sequences, 0 .. 4096 */
     int32_t hq, hkv;               /* hq a multiple of hkv */
     int32_t head_dim;              /* 64 or 128 */
-    float sm_scale;                /* > 0 */
-    float logit_cap;               /* soft cap, used when > 0 */
+    float sm_scale;                /* > 0, finite */
+    float logit_cap;               /* soft cap, used when > 0; finite */
     const void* q;                 /* token t, head h at q + t*q_stride + h*head_dim (elements) */
     const void* k;
     const void* v;

@@ -242,3 +242,17 @@ def test_calls_refuse_outputs_that_share_memory(lib):
     for bad in ("pool", "req_to_token", "req_pool_indices", "seq_lens"):
         assert lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **(p | {"out": p[bad] + 4})))) == 1, bad
     assert lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **p))) == 3 == lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **(p | {"out": p["q"]}))))
+
+
+def test_numbers_that_are_not_finite_are_refused(lib):
+    """An infinite soft cap would make every logit undefined, an infinite base of the angles leave a pair unturned."""
+    for x in (float("inf"), float("nan")):
+        for bad in (dict(logit_cap=x), dict(sm_scale=x), dict(rope_base=x), dict(rope_scale=x)):
+            assert lib.ts_quant_attend(C.byref(_attend(device=NOWHERE, **(_far(names="q pool req_to_token req_pool_indices seq_lens out workspace") | bad)))) == 1, bad
+        for bad in (dict(logit_cap=x), dict(sm_scale=x)):
+            assert lib.ts_prompt_attend(C.byref(_prompt(device=NOWHERE, **(_far(names="q k v cu_seqlens out") | bad)))) == 1, bad
+        for bad in (dict(rope_base=x), dict(rope_scale=x)):
+            p = _far(names="q k positions q_out k_out")
+            assert lib.ts_norm_rotate(C.byref(_norm(device=NOWHERE, **(p | bad)))) == 1, bad
+            assert lib.ts_norm_rotate(C.byref(_norm(device=NOWHERE, **(p | bad | {"positions": None})))) == 3, bad
+    assert lib.ts_prompt_attend(C.byref(_prompt(device=NOWHERE, logit_cap=-1.0, **_far(names="q k v cu_seqlens out")))) == 3

@@ -185,7 +185,7 @@ extern "C" int ts_norm_rotate(const ts_norm_rotate_args* a) {
     if (a->tokens < 0 || a->hq < 1 || a->hkv < 1 || a->hq > 1024 || a->hkv > 1024) return TS_ERR_INVALID_ARG;
     if (a->q_stride < (int64_t)a->hq * a->head_dim || a->k_stride < (int64_t)a->hkv * a->head_dim) return TS_ERR_INVALID_ARG;
     if (!(a->eps >= 0.f)) return TS_ERR_INVALID_ARG;
-    if (a->positions && (!(a->rope_base > 0.0) || !(a->rope_scale > 0.0))) return TS_ERR_INVALID_ARG;
+    if (a->positions && (!positive(a->rope_base) || !positive(a->rope_scale))) return TS_ERR_INVALID_ARG;
     if (a->tokens == 0) return TS_OK;
     if (!a->q || !a->k || !a->q_out || !a->k_out) return TS_ERR_INVALID_ARG;
     {

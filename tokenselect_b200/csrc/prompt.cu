@@ -896,7 +896,7 @@ extern "C" int ts_prompt_attend(const ts_prompt_args* a) {
     if (a->head_dim != 64 && a->head_dim != 128) return TS_ERR_UNSUPPORTED;
     if (a->tokens < 0 || a->batch < 0 || a->batch > kPromptMaxBatch || a->hq < 1 || a->hkv < 1 || a->hq > 8192 || a->hq % a->hkv != 0) return TS_ERR_INVALID_ARG;
     if (a->q_stride < (int64_t)a->hq * a->head_dim || a->k_stride < (int64_t)a->hkv * a->head_dim || a->v_stride < (int64_t)a->hkv * a->head_dim) return TS_ERR_INVALID_ARG;
-    if (!(a->sm_scale > 0.f) || !isfinite(a->sm_scale)) return TS_ERR_INVALID_ARG;
+    if (!positive(a->sm_scale) || !isfinite(a->logit_cap)) return TS_ERR_INVALID_ARG;
     if (a->tokens == 0 || a->batch == 0) return TS_OK;
     if (!a->q || !a->k || !a->v || !a->cu_seqlens || !a->out) return TS_ERR_INVALID_ARG;
     const int es = a->dtype == TS_DTYPE_BF16 ? 2 : 4;

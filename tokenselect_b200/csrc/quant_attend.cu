@@ -923,10 +923,10 @@ extern "C" int ts_quant_attend(const ts_quant_attend_args* a) {
     if (a->head_dim != 64 && a->head_dim != 128) return TS_ERR_UNSUPPORTED;
     if (a->batch < 0 || a->batch > kQaMaxBatch || a->hq < 1 || a->hkv < 1 || a->hkv > 1024 || a->hq % a->hkv != 0) return TS_ERR_INVALID_ARG;
     if (a->hq / a->hkv > 8) return TS_ERR_UNSUPPORTED;
-    if (!(a->rope_base > 0.0) || !(a->rope_scale > 0.0) || !power_of_two(a->k_scale) || !power_of_two(a->v_scale)) return TS_ERR_INVALID_ARG;
+    if (!positive(a->rope_base) || !positive(a->rope_scale) || !power_of_two(a->k_scale) || !power_of_two(a->v_scale)) return TS_ERR_INVALID_ARG;
     if (a->max_reqs < 1 || a->max_ctx < 0 || a->req_to_token_stride < 0 || a->pool_rows < 1) return TS_ERR_INVALID_ARG;
     if (a->max_ctx > (1ll << 31) - kUnit || (a->max_ctx + kUnit - 1) / kUnit * a->batch >= (1ll << 31)) return TS_ERR_INVALID_ARG;   // units are counted in 32 bits
-    if (!(a->sm_scale > 0.f) || !isfinite(a->sm_scale)) return TS_ERR_INVALID_ARG;
+    if (!positive(a->sm_scale) || !isfinite(a->logit_cap)) return TS_ERR_INVALID_ARG;
     if (a->batch == 0) return TS_OK;
     if (!a->q || !a->pool || !a->req_to_token || !a->req_pool_indices || !a->seq_lens || !a->out || !a->workspace) return TS_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(a->pool) % 16 != 0 || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return TS_ERR_INVALID_ARG;

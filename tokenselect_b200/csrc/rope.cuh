@@ -137,6 +137,7 @@ __device__ __forceinline__ void wait_phase(uint32_t bar, uint32_t parity, int* s
     }
 }
 
+inline bool positive(double x) { return x > 0.0 && isfinite(x); }
 inline bool power_of_two(float g) {
     int e;
     return g >= 2.3283064365386963e-10f && g <= 4294967296.f && frexpf(g, &e) == 0.5f;
