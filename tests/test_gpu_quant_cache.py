@@ -455,3 +455,27 @@ def test_type_of_what_is_read():
     for kw in ({"k": given}, {"v": given}):
         with pytest.raises(ValueError, match="dtype"):
             qc.kv4_read(pool, rows, BF16, **kw)
+
+
+@pytest.mark.parametrize("octaves", [24.5, 25.5, 28.0])
+def test_many_small_weights_beside_a_large_one(octaves):
+    """Every 2000th row holds 2^24 to 2^28 times the weight of the rows behind it, and its value is 0: what the others add up to
+    is not lost.  (Each CTA's rows begin with a large one.  Keys and queries lie in the slowest pair of a base so large that
+    nothing turns.)"""
+    heads, d, every, v1 = 8, 64, 2000, 3.0
+    n = torch.cuda.get_device_properties(0).multi_processor_count * every
+    k, v = torch.zeros(2, heads, d), torch.zeros(2, heads, d)
+    k[0, :, d // 2 - 1], v[1] = 1.0, v1
+    pool = ref.pack(k, v)                                                    # row 0: a large weight; row 1: a key of zeros
+    kh, vh = ref.unpack(pool)
+    table = (torch.arange(n) % every != 0).int()[None]
+    q = torch.zeros(1, heads, d)
+    q[:, :, d // 2 - 1] = 1.0
+    scale = octaves * 0.6931471805599453 / float(kh[0, 0, d // 2 - 1])
+    out = qc.kv4_attend(q.view(1, -1).to(BF16).cuda(), pool.cuda(), table.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda"),
+                        torch.tensor([n], dtype=torch.int32, device="cuda"), scale, 1e30).cpu().double()
+    small = (every - 1) * 2.0 ** -octaves
+    want = small / (1.0 + small) * float(vh[1, 0, 0])
+    e = torch.tensor(6 * 5 * 2.0 ** -11 * octaves * 0.6931471805599453)      # |q_i| = 1, scale |k_i| = the logit
+    tol = want * (2.0 ** -8 + float(torch.exp(2 * e)) - 1 + 2.0 ** -10) + every * 2.0 ** -32 * v1
+    assert float((out - want).abs().max()) <= tol, (want, float(out[0, 0]), tol)

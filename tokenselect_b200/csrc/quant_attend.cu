@@ -272,6 +272,10 @@ struct QtLaunch {
     static constexpr int kComputeRegs = PIECE == 0 ? 224 : 200;        // 2 * 224 + 56 = 3 * 168; 2 * 200 + 2 * 56 = 4 * 128 a thread
 };
 constexpr int kQtMacro = 8;                                    // units of a macro tile
+// Weights enter the second product in fp16, whose smallest number is 2^-24 and largest below 2^16.  They are taken 2^7 times as
+// large as their reference says (in the sum too), so that what a warp loses of many small weights beside a large one is
+// at most 2^-32 of it each, and not 2^-25.
+constexpr float kQtLift = 7.f;
 // Stages of a ring: a step holds two while the two behind it arrive, so fewer than four would wait for themselves.  And never
 // fewer than warps that fill it in turn: a warp asks for the stage's release before last with the same parity, and knows that one
 // to have happened because it filled a stage that many units ago.
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(QtLaunch<PIECE>::kThreads, 1) quant_attend_tc_
                     x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, off));
                     x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, off));
                 }
-                // the reference maximum moves only when a row grew by more than 2^8: weights stay below 256
+                // the reference maximum moves only when a row grew by more than 2^8: weights stay below 2^(8 + kQtLift)
                 if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f)) {
                     const float n0 = fmaxf(fmaxf(m0, x0), -1e30f), n1 = fmaxf(fmaxf(m1, x1), -1e30f);
                     const float c0 = exp2_fast(m0 - n0), c1 = exp2_fast(m1 - n1);
@@ -692,7 +696,7 @@ __global__ void __launch_bounds__(QtLaunch<PIECE>::kThreads, 1) quant_attend_tc_
                     if (j >= cnt) break;
                     float pe[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) pe[e] = exp2_fast(fmaf(sc[j][e], (e & 1) ? k1 : k0, (e & 1) ? -m1 : -m0));
+                    for (int e = 0; e < 4; ++e) pe[e] = exp2_fast(fmaf(sc[j][e], (e & 1) ? k1 : k0, kQtLift - ((e & 1) ? m1 : m0)));
                     l0 += pe[0] + pe[2];
                     l1 += pe[1] + pe[3];
                     const uint32_t b0 = transpose8(pack2(pe[0], pe[1])), b1 = transpose8(pack2(pe[2], pe[3]));
