@@ -426,3 +426,51 @@ def test_sequences_of_bounds_out_of_order_share_no_token(dtype):
             outs.append(out)
         assert torch.equal(outs[0], outs[1]), case
         assert bool((outs[0][:good[0]] == 7.0).all()) and bool((outs[0][good[-1]:] == 7.0).all()) and not bool((outs[0][good[0]:good[-1]] == 7.0).any())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinite_keys_in_fp32(d):
+    """The check mode gives the same: undefined, a weight of zero, or no softmax at all."""
+    n, hq, hkv = 200, 2, 1
+    q, k, v, cu = _prompt_case(61, hq, hkv, d, [n], F32)
+    one, two, all_ = k.clone(), k.clone(), k.clone()
+    one[6, 0, 5] = float("inf")
+    two[70, 0, 5], two[70, 0, 6] = float("inf"), -float("inf")
+    all_[:, 0, 5] = -float("inf")
+    for k2 in (one, two, all_):
+        out = prompt.prompt_attend(q.cuda(), k2.cuda(), v.cuda(), cu.cuda(), d ** -0.5)
+        _matches(out, *ref.attend(q, k2, v, ref.causal([n], n), d ** -0.5))
+
+
+def test_a_captured_decode_step_over_a_4bit_cache():
+    """Norm, rows written, attention and rows read back in one graph: a replay follows new contents of every input, and gives
+    what the calls give one by one."""
+    hq, hkv, d, base, batch = 8, 2, 128, 5e5, 3
+    g = torch.Generator().manual_seed(71)
+    qkv = torch.randn(batch, (hq + 2 * hkv) * d, generator=g).to(BF16).cuda()
+    q, k, v = (qkv[:, a * d:b * d].view(batch, -1, d) for a, b in ((0, hq), (hq, hq + hkv), (hq + hkv, hq + 2 * hkv)))
+    w = torch.ones(d, dtype=BF16, device="cuda")
+    start = torch.randint(0, 120, (200, hkv, qc.kv4_row_bytes(d)), dtype=torch.uint8, generator=g).cuda()      # (no NaN scale)
+    table = torch.randperm(200, generator=g).int().view(1, 200).expand(batch, 200).cuda()
+    loc, lens, slots = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([5, 6, 7], [17, 200, 33], [2, 0, 1]))
+
+    def step(pool):
+        qn, kn = prompt.norm_rotate(q, k, None, q_weight=w, k_weight=w)
+        qc.kv4_write(pool, kn, v, loc)
+        out = qc.kv4_attend(qn.view(batch, hq * d), pool, table, slots, lens, 0.1, base)
+        return (out, *qc.kv4_read(pool, loc))
+
+    step(start.clone())
+    pool = start.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(pool)
+    for turn in range(3):
+        qkv.copy_(torch.randn(qkv.shape, generator=g).to(BF16))
+        loc.copy_(torch.tensor([9 + turn, 50 + turn, 80 + turn], dtype=torch.int32))
+        lens.copy_(torch.tensor([1 + turn, 0, 190 + turn], dtype=torch.int32))
+        pool.copy_(start)
+        graph.replay()
+        other = start.clone()
+        assert all(torch.equal(a, b) for a, b in zip(res, step(other))) and torch.equal(pool, other)
