@@ -388,7 +388,8 @@ int ts_quant_read(const ts_quant_rows_args* args);
  * A request of length 0 gets zeros.  A length below 0 or above max_ctx, or a request slot outside [0, max_reqs), gives zeros
  * and is reported (TS_ERR_BAD_LENGTH); a row outside the pool counts as a row of zeros and is reported (TS_ERR_BAD_SLOT).
  * In bf16 the rotated keys and queries and the softmax weights enter the products in fp16 (the queries scaled by a power of
- * two into its range), all sums are fp32; in fp32 everything is fp32.
+ * two into its range; cosines and sines of a key's place among 128 in fp16 too; a weight below 2^-32 of the largest that a
+ * share of the rows met counts in the sum alone), all sums are fp32; in fp32 everything is fp32.
  * `workspace` holds the partial results of one call (ts_quant_attend_workspace() bytes, any contents): calls that may run
  * at the same time need one each.  It shares no byte with the call's tensors, nor `out` with any but q (TS_ERR_INVALID_ARG).
  */
@@ -428,7 +429,7 @@ int ts_quant_attend(const ts_quant_attend_args* args);
  * RMS norm of every query and key head and the rotation of both, in one pass over them:
  *   y = x * rsqrt(mean(x^2) + eps) * weight        (no norm where the weight is NULL)
  *   (y_i, y_{i+head_dim/2}) turned by position * rope_base^(-2i/head_dim) / rope_scale    (no rotation where positions is NULL)
- * in fp32, rounded once.  k_plain, if not NULL, takes the normed keys before the rotation: what a cache of un-rotated keys
+ * in fp32 (cosines and sines to 2^-20 where the tensors are bf16), rounded once.  k_plain, if not NULL, takes the normed keys before the rotation: what a cache of un-rotated keys
  * keeps.  Outputs are contiguous [tokens, heads, head_dim]; an output may be the whole place of the (contiguous) input that it is
  * made of, and shares no byte with another tensor of the call otherwise (TS_ERR_INVALID_ARG).
  */
@@ -465,7 +466,8 @@ int ts_norm_rotate(const ts_norm_rotate_args* args);
  * starts behind all before it (no token belongs to two), and is reported (TS_ERR_BAD_LENGTH).  Rows of `out` that belong to no sequence (those behind the last one among them) are left as
  * they were.  No value of one sequence reaches another, infinities and NaN included; inside
  * a sequence they reach the tokens that attend to them.
- * In bf16 the softmax weights enter the second product in bf16, all sums are fp32; in fp32 everything is fp32.
+ * In bf16 the softmax weights enter the second product in bf16 (the sum takes them as they were), a quarter of the exponentials
+ * is a polynomial's, to 7.5e-5 of itself, all sums are fp32; in fp32 everything is fp32.
  * bf16: q, k, v start on multiples of 16 bytes and their strides are multiples of 8 elements; out starts on a multiple of
  * 16 bytes.  fp32: on multiples of 16 bytes, strides multiples of 4 elements.  (TS_ERR_INVALID_ARG otherwise.)
  */

@@ -31,7 +31,7 @@ struct NormParams {
     void* k_out;
     void* k_plain;
     int hq, hkv;
-    unsigned groups_q, per_token;                              // groups of four heads: of the queries, of a token
+    unsigned groups_q, per_token;                              // groups of kNormHeads heads: of the queries, of a token
     unsigned long long groups;
     float eps;
     TurnFreqs freqs;

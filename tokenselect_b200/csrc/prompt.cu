@@ -292,7 +292,9 @@ cudaError_t launch_prompt_plain(const PromptParams& p, cudaStream_t stream) {
 //    parts.  One pair of columns in four takes its exponentials on the multipliers: the exponential unit alone would need as
 //    long as the tensor pipe.  (1190 -> 1283; without the multipliers 1239, with one pair in three 1246, in eight 1230, P in
 //    one part 1218.)
-//  * now: power (1.59 GHz of 1.965 during the run); the tensor pipe is busy for 66 % of the cycles.
+//  * now: that way still (the tensor pipe is busy for 65 % of the cycles, the exponential unit for 49 %), and the clock, which the
+//    card's power limit takes from 1.965 to 1.58 GHz when the kernel runs on (435 us after a pause, 516 us then, whether on one
+//    input or on changing ones).
 //
 // One thread requests tiles (tiled copies, 128-byte swizzle): Q, and K and V blocks through a ring of five.  It runs ahead
 // into the CTA's next tile, of which it leaves the place in a two-entry queue.  Tiles are dealt out in the order of their

@@ -2,8 +2,9 @@
 //
 // Per block of sixteen elements x: scale = E4M3(min(max|x| / (6 g), 448)), code = E2M1(x / (g scale)), value = code scale g.
 //
-// What bounds both: HBM (a bf16 row of 2 KB at eight heads becomes 1152 bytes with its V), and for the rows of a decode
-// step the launch.  One thread takes one block: 32 bytes of bf16 or 64 of fp32 on one side, eight bytes of codes and one
+// What bounds both: HBM (a bf16 row of 2 KB at eight heads becomes 1152 bytes with its V) and, as they are, instructions and the
+// waits for loads (16385 rows of eight heads: writing 25 us, issue slots 67 % busy, reading 18 us, 64 %; 13 us of bytes each); for
+// the rows of a decode step the launch.  One thread takes one block: 32 bytes of bf16 or 64 of fp32 on one side, eight bytes of codes and one
 // scale on the other, so the maximum needs no exchange and neighbouring lanes touch neighbouring bytes on both sides.
 //
 // Rounding is decided exactly.  g is a power of two, so x / g is exact; max|x| / 6 is IEEE-divided, and a quotient that

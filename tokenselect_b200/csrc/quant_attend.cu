@@ -852,7 +852,8 @@ __global__ void __launch_bounds__(32 * WARPS) quant_merge_kernel(const __grid_co
 }
 
 // Pieces the sequence of units is cut into: for the tensor cores one CTA per SM, eight warps over at most eight KV heads
-// each; for the CUDA cores what fits an SM.
+// each; for the CUDA cores what fits an SM.  (With three or more blocks of heads the CTAs may be a few more than the SMs: 24 heads
+// make 3 x 50, 40 heads 5 x 30, and the last two run behind the others.)
 int tc_head_blocks(int hkv) { return (hkv + kQtWarps - 1) / kQtWarps; }
 int attend_pieces(int dtype, int hkv, int sms) {
     return dtype == TS_DTYPE_BF16 ? (sms + tc_head_blocks(hkv) - 1) / tc_head_blocks(hkv) : 4 * sms;
