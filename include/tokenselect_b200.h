@@ -429,9 +429,10 @@ int ts_quant_attend(const ts_quant_attend_args* args);
  * RMS norm of every query and key head and the rotation of both, in one pass over them:
  *   y = x * rsqrt(mean(x^2) + eps) * weight        (no norm where the weight is NULL)
  *   (y_i, y_{i+head_dim/2}) turned by position * rope_base^(-2i/head_dim) / rope_scale    (no rotation where positions is NULL)
- * in fp32 (cosines and sines to 2^-20 where the tensors are bf16), rounded once.  k_plain, if not NULL, takes the normed keys before the rotation: what a cache of un-rotated keys
- * keeps.  Outputs are contiguous [tokens, heads, head_dim]; an output may be the whole place of the (contiguous) input that it is
- * made of, and shares no byte with another tensor of the call otherwise (TS_ERR_INVALID_ARG).
+ * in fp32 (cosines and sines to 2^-20 where the tensors are bf16), rounded once.  k_plain, if not NULL, takes the normed keys
+ * before the rotation: what a cache of un-rotated keys keeps.  Outputs are contiguous [tokens, heads, head_dim]; an output may be
+ * the whole place of the (contiguous) input that it is made of, and shares no byte with another tensor of the call otherwise
+ * (TS_ERR_INVALID_ARG).
  */
 typedef struct ts_norm_rotate_args {
     uint32_t struct_size;          /* sizeof(ts_norm_rotate_args), checked */
@@ -463,9 +464,9 @@ int ts_norm_rotate(const ts_norm_rotate_args* args);
  * cu_seqlens[b] .. cu_seqlens[b+1]-1; token i attends to the tokens of its own sequence up to itself.  q and k come already
  * rotated (ts_norm_rotate).  Query head h reads KV head h / (hq/hkv).  Lengths of zero and one are lengths like any other.
  * cu_seqlens is read on the device; a bound outside [0, tokens] or below one before it ends the sequence there, the next one
- * starts behind all before it (no token belongs to two), and is reported (TS_ERR_BAD_LENGTH).  Rows of `out` that belong to no sequence (those behind the last one among them) are left as
- * they were.  No value of one sequence reaches another, infinities and NaN included; inside
- * a sequence they reach the tokens that attend to them.
+ * starts behind all before it (no token belongs to two), and is reported (TS_ERR_BAD_LENGTH).  Rows of `out` that belong to no
+ * sequence (those behind the last one among them) are left as they were.  No value of one sequence reaches another, infinities
+ * and NaN included; inside a sequence they reach the tokens that attend to them.
  * In bf16 the softmax weights enter the second product in bf16 (the sum takes them as they were), a quarter of the exponentials
  * is a polynomial's, to 7.5e-5 of itself, all sums are fp32; in fp32 everything is fp32.
  * bf16: q, k, v start on multiples of 16 bytes and their strides are multiples of 8 elements; out starts on a multiple of

@@ -470,8 +470,8 @@ __device__ __noinline__ void mend_rows(const PromptParams& p, int first, int row
     __syncwarp();
 }
 
-// 2^x of two numbers on the multipliers, for x >= -125 (below, and for minus infinity and NaN, 2^-125): 2^n 2^f with n the nearest whole number and 2^f a
-// polynomial of degree 3 (Remez exchange: 7.5e-5 relative on [-1/2, 1/2], a twentieth of the weight's rounding to bf16).
+// 2^x of two numbers on the multipliers, for x >= -125 (below, and for minus infinity and NaN, 2^-125): 2^n 2^f with n the
+// nearest whole number and 2^f a polynomial of degree 3 (Remez exchange: 7.5e-5 relative on [-1/2, 1/2], a twentieth of the weight's rounding to bf16).
 __device__ __forceinline__ uint64_t exp2_f32x2(uint64_t x) {
     float a, b;
     unpack_f32x2(x, a, b);

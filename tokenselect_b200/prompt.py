@@ -93,10 +93,10 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens:
     """Causal attention of packed prompts: ``q [tokens, heads, head_dim]``, ``k, v [tokens, kv_heads, head_dim]``, q and
     k rotated; sequence ``b`` is the tokens ``cu_seqlens[b] .. cu_seqlens[b+1] - 1`` (int32 ``[sequences + 1]`` on the
     device, lengths of zero allowed).  Query head ``h`` reads KV head ``h // group``.  Returns ``[tokens, heads,
-    head_dim]`` (``out`` shares no memory with the inputs); rows behind the last sequence are left as they were in ``out``.  The tensors start on 16 bytes and
-    their tokens lie a multiple of 16 bytes apart (slices of a fused projection do).  ``status`` (optional, int32) is
-    set when a bound of ``cu_seqlens`` makes no sense; the sequence then ends where it still does, and the next one starts
-    behind all before it."""
+    head_dim]`` (``out`` shares no memory with the inputs); rows behind the last sequence are left as they were in ``out``.
+    The tensors start on 16 bytes and their tokens lie a multiple of 16 bytes apart (slices of a fused projection do).
+    ``status`` (optional, int32) is set when a bound of ``cu_seqlens`` makes no sense; the sequence then ends where it
+    still does, and the next one starts behind all before it."""
     dev, dtype, shape = q.get_device(), q.dtype, q.shape
     if len(shape) != 3:
         raise ValueError("q must be [tokens, heads, head_dim]")
